@@ -228,6 +228,98 @@ def paged_decode(q, k_cache, v_cache, block_tables, ctx_lens, out, num_heads, sc
     return ref.paged_decode(q, k_cache, v_cache, block_tables, ctx_lens, out, num_heads, scale)
 
 
+# ----------------------------------------------------------------- 4-bit KV cache
+
+# Channels that share one scale and zero point; more channels, fewer bytes:
+# 80 / 72 / 68 bytes per token, head and K or V (bf16: 256).
+KV4_GROUPS = (32, 64, 128)
+
+
+def kv4_record_bytes(group: int) -> int:
+    """Bytes of 16 tokens of one head (K or V) of a 4-bit cache."""
+    if group not in KV4_GROUPS:
+        raise ValueError(f"kv4 group must be one of {KV4_GROUPS}, got {group}")
+    return 1024 + 64 * (128 // group)
+
+
+def kv4_cache_shape(pages: int, num_kv_heads: int, block_size: int, group: int) -> tuple[int, ...]:
+    """Shape of one layer's uint8 cache: ``[pages, kv heads, block_size / 16,
+    2 (K, V), record bytes]``; a page of a head is one contiguous run."""
+    if block_size <= 0 or block_size % 16:
+        raise ValueError("block_size must be a positive multiple of 16")
+    return (pages, num_kv_heads, block_size // 16, 2, kv4_record_bytes(group))
+
+
+def kv4_write(k, v, cache, slot_mapping):
+    """Quantise the rows ``k`` / ``v`` (bf16 ``[T, Hkv * 128]`` or ``[T, Hkv,
+    128]``, any row stride) into the 4-bit ``cache`` at ``slot_mapping`` (int64
+    ``[T]``; distinct slots; a negative one is not cached).
+
+    Groups of 32, 64 or 128 channels (by the cache's record size) share a bf16
+    scale and an fp16 zero point. Magnitudes above 8192 saturate, a NaN is
+    stored as 0."""
+    if cache.is_cuda:
+        _native().kv4_write(k, v, cache, slot_mapping)
+        return
+    ref.kv4_write(k, v, cache, slot_mapping)
+
+
+def kv4_read(cache, slots):
+    """(K, V) rows bf16 ``[T, Hkv * 128]`` that ``slots`` (int64 ``[T]``) of a
+    4-bit cache stand for; zeros for a negative slot."""
+    if cache.is_cuda:
+        return _native().kv4_read(cache, slots)
+    return ref.kv4_read(cache, slots)
+
+
+def kv4_workspace(device):
+    """Workspace of :func:`paged_decode4` and :func:`paged_prefill4`: one per
+    stream, for all layers and any batch (calls that may overlap on the GPU need
+    one each)."""
+    device = torch.device(device)
+    n = _native(0).kv4_workspace_bytes() if device.type == "cuda" else 0
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws):
+    """:func:`paged_decode` over a 4-bit cache: ``q`` / ``out`` bf16 ``[B, Hq *
+    128]`` (row strides free; ``q`` rows 16-byte aligned), ``block_tables`` int32
+    ``[B, pages]``, ``ctx_lens`` int32 ``[B]`` (0: zeros out), 1 to 16 query heads
+    per KV head. Lengths are read on the device, so a captured call serves any.
+    ``ws`` from :func:`kv4_workspace`."""
+    if cache.is_cuda:
+        LAUNCHES[0] += _native(0).paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws)
+        return out
+    return ref.paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale)
+
+
+def paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale, ws):
+    """:func:`paged_prefill` over a 4-bit cache."""
+    return ref.paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale)
+
+
+def copy_pages(caches, src, dst):
+    """Copy pages ``src[i] -> dst[i]`` (host lists) of every cache in ``caches``
+    (contiguous tensors of one shape whose dimension 0 is the page: bf16 K / V or
+    4-bit), e.g. to fork a request's partly filled page or to compact the pool.
+    The copies run in no order: a destination may appear once and may not be a
+    source."""
+    if len(src) != len(dst):
+        raise ValueError(f"copy_pages: {len(src)} sources for {len(dst)} destinations")
+    if not src or not caches:
+        return
+    pages = caches[0].shape[0]
+    to = set(dst)
+    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= pages:
+        raise ValueError(f"copy_pages: page ids must be in [0, {pages})")
+    if len(to) != len(dst) or not to.isdisjoint(src):
+        raise ValueError("copy_pages: a destination may appear once and may not be a source")
+    if caches[0].is_cuda:
+        LAUNCHES[0] += _native(0).copy_pages(caches, src, dst)
+        return
+    ref.copy_pages(caches, src, dst)
+
+
 # ----------------------------------------------------------------- trainer attention
 
 def dense_attn_tiles(starts, lens, device, bm: int = 64) -> torch.Tensor:

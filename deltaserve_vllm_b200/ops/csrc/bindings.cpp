@@ -45,14 +45,23 @@ void dsv_adamw_slice_bcast(torch::Tensor p, torch::Tensor g, torch::Tensor m, to
                            double eps, double wd, int64_t step, int64_t rank, int64_t world, torch::Tensor table);
 void dsv_ce_merge(torch::Tensor stats, int64_t n_tiles, torch::Tensor tgt, torch::Tensor part);
 void dsv_ce_finalize(torch::Tensor parts, torch::Tensor labels, torch::Tensor lse, torch::Tensor loss);
+void dsv_kv4_write(torch::Tensor k, torch::Tensor v, torch::Tensor cache, torch::Tensor slots);
+std::tuple<torch::Tensor, torch::Tensor> dsv_kv4_read(torch::Tensor cache, torch::Tensor slots);
+int64_t dsv_copy_pages(std::vector<torch::Tensor> caches, std::vector<int64_t> src, std::vector<int64_t> dst);
+int64_t dsv_kv4_workspace_bytes();
+int64_t dsv_paged_decode4(torch::Tensor q, torch::Tensor cache, torch::Tensor tables, torch::Tensor ctx,
+                          torch::Tensor out, int64_t heads, double scale, torch::Tensor ws);
 int64_t dsv_read_error_gemm(bool clear);
 int64_t dsv_read_error_attn_bwd(bool clear);
 int64_t dsv_read_error_tp_bwd(bool clear);
 int64_t dsv_read_error_attn_tc(bool clear);
 int64_t dsv_read_error_attn_bwd_tc(bool clear);
+int64_t dsv_read_error_kv4_cache(bool clear);
+int64_t dsv_read_error_kv4_decode(bool clear);
 static int64_t dsv_read_error(bool clear) {
-  const int64_t codes[5] = {dsv_read_error_gemm(clear), dsv_read_error_attn_bwd(clear), dsv_read_error_tp_bwd(clear),
-                            dsv_read_error_attn_tc(clear), dsv_read_error_attn_bwd_tc(clear)};
+  const int64_t codes[] = {dsv_read_error_gemm(clear), dsv_read_error_attn_bwd(clear), dsv_read_error_tp_bwd(clear),
+                           dsv_read_error_attn_tc(clear), dsv_read_error_attn_bwd_tc(clear),
+                           dsv_read_error_kv4_cache(clear), dsv_read_error_kv4_decode(clear)};
   for (int64_t c : codes)
     if (c != 0) return c;
   return 0;
@@ -144,6 +153,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_fwd_dense_tc", &dsv_attn_fwd_dense_tc,
         "varlen causal GQA attention forward on packed rows, tcgen05 + TMA (optional lse / rowsum(dO*O))");
   m.def("paged_decode", &dsv_paged_decode, "paged split-KV GQA decode attention");
+  m.def("kv4_write", &dsv_kv4_write, "quantise K / V rows into a 4-bit paged cache");
+  m.def("kv4_read", &dsv_kv4_read, "bf16 K / V rows of slots of a 4-bit paged cache");
+  m.def("copy_pages", &dsv_copy_pages, "copy pages of every layer's cache; returns the launches");
+  m.def("kv4_workspace_bytes", &dsv_kv4_workspace_bytes, "bytes of the attention workspace of the 4-bit cache");
+  m.def("paged_decode4", &dsv_paged_decode4, "decode attention over a 4-bit paged cache; returns the launches");
   m.def("attn_bwd", &dsv_attn_bwd, "varlen causal GQA attention backward (dQ, dK, dV)");
   m.def("attn_fwd_dense", &dsv_attn_fwd_dense, "varlen causal GQA attention forward on packed rows");
   m.def("rms_norm", &dsv_rms_norm, "RMSNorm / fused residual add + RMSNorm (+ row capture)");

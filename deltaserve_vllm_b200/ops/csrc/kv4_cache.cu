@@ -1,0 +1,309 @@
+// Writing, reading and copying the 4-bit KV cache (format: kv4.cuh).
+//
+// The reference project keeps its cache in the serving library's bf16 pages and
+// has no counterpart of these kernels.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "kv4.cuh"
+
+namespace dsv {
+
+struct Kv4RowsArgs {
+  const __nv_bfloat16* k;   // [T, Hkv, 128], strides in elements
+  const __nv_bfloat16* v;
+  int64_t k_row, k_head, v_row, v_head;
+  uint8_t* cache;
+  const int64_t* slots;     // [T], negative = not cached
+  int64_t num_slots;        // pages * page size
+  int rows, heads, page;
+  __nv_bfloat16* k_out;     // read: contiguous [T, Hkv * 128]
+  __nv_bfloat16* v_out;
+};
+
+// Address of the K record of a slot's token and head, and the token's place in it.
+template <int NG>
+__device__ __forceinline__ uint8_t* kv4_record_of(const Kv4RowsArgs& a, int64_t slot, int head, int& r) {
+  const int64_t page = slot / a.page;
+  const int off = (int)(slot - page * a.page);
+  r = off & 15;
+  return a.cache + (size_t)(((page * a.heads + head) * (a.page / 16) + (off >> 4)) * 2) * kv4_record(NG);
+}
+
+// Quantise this lane's 4 channels (4 lane .. + 3) of a row; the group's
+// statistics come from the 32 / NG lanes that share it. Returns the four codes
+// as nibbles and the group's (scale, zero) word. Each step is rounded as the
+// format says (no contraction), so any implementation of it gives these bits.
+template <int NG>
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[4], uint32_t& word) {
+  float y[4], lo = 0.f, hi = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -KV4_LIMIT), KV4_LIMIT) : 0.f;
+    lo = fminf(lo, y[e]);
+    hi = fmaxf(hi, y[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < 32 / NG; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
+  if (s < KV4_TINY) s = 0.f;
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  const __half zh = __float2half_rn(__fmul_rn(lo, inv));
+  const float z = __half2float(zh);
+  word = __float_as_uint(s) | __half_as_ushort(zh);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float c = fminf(fmaxf(rintf(__fsub_rn(__fmul_rn(y[e], inv), z)), 0.f), 15.f);
+    codes |= (uint32_t)c << (4 * e);
+  }
+  return codes;
+}
+
+__device__ __forceinline__ void kv4_load4(const __nv_bfloat16* p, bool vec, float (&x)[4]) {
+  if (vec) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(w.x << 16);
+    x[1] = __uint_as_float(w.x & 0xffff0000u);
+    x[2] = __uint_as_float(w.y << 16);
+    x[3] = __uint_as_float(w.y & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = bf2f(p[e]);
+  }
+}
+
+// One warp = one (token, head), K then V; lane owns 4 channels.
+template <int NG>
+__global__ void __launch_bounds__(256) kv4_write_kernel(Kv4RowsArgs a, bool vec) {
+  const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
+  const int lane = threadIdx.x & 31;
+  if (w >= (int64_t)a.rows * a.heads) return;
+  const int row = (int)(w / a.heads), head = (int)(w % a.heads);
+  const int64_t slot = a.slots[row];
+  if (slot < 0) return;
+  if (slot >= a.num_slots) {
+    if (lane == 0) set_error(kErrShape);
+    return;
+  }
+  int r;
+  uint8_t* krec = kv4_record_of<NG>(a, slot, head, r);
+  uint8_t* vrec = krec + kv4_record(NG);
+  float x[4];
+  uint32_t word;
+  kv4_load4(a.k + row * a.k_row + head * a.k_head + 4 * lane, vec, x);
+  uint32_t c = kv4_quantise<NG>(x, word);
+  // K: lane's codes are half a word of channels 32 i + 8 t + 0..7
+  const uint32_t up = __shfl_down_sync(0xffffffffu, c, 1);
+  if (!(lane & 1))
+    *reinterpret_cast<uint32_t*>(krec + 64 * r + 16 * (lane % 8 / 2) + 4 * (lane / 8)) = c | up << 16;
+  if (lane % (32 / NG) == 0)
+    *reinterpret_cast<uint32_t*>(krec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r) = word;
+  kv4_load4(a.v + row * a.v_row + head * a.v_head + 4 * lane, vec, x);
+  c = kv4_quantise<NG>(x, word);
+  // V: channels g and g + 8 of a 16-channel tile share a byte; lane ^ 2 holds the other half
+  const uint32_t hi = __shfl_down_sync(0xffffffffu, c, 2);
+  if (!(lane & 2)) {
+    uint8_t* dst = vrec + 512 * (lane / 16) + 16 * (r % 8 / 2) + 4 * (lane / 4 % 4) + (r / 8) + 2 * (r % 2);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      dst[64 * (4 * (lane & 1) + e)] = (uint8_t)((c >> (4 * e) & 15u) | (hi >> (4 * e) & 15u) << 4);
+  }
+  if (lane % (32 / NG) == 0)
+    *reinterpret_cast<uint32_t*>(vrec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r) = word;
+}
+
+// The values a slot's codes stand for, as bf16 rows; zeros for a negative slot.
+template <int NG>
+__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4RowsArgs a) {
+  const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
+  const int lane = threadIdx.x & 31;
+  if (w >= (int64_t)a.rows * a.heads) return;
+  const int row = (int)(w / a.heads), head = (int)(w % a.heads);
+  const int64_t slot = a.slots[row];
+  uint2 ko = make_uint2(0, 0), vo = make_uint2(0, 0);
+  if (slot >= a.num_slots) {
+    if (lane == 0) set_error(kErrShape);
+  } else if (slot >= 0) {
+    int r;
+    const uint8_t* krec = kv4_record_of<NG>(a, slot, head, r);
+    const uint8_t* vrec = krec + kv4_record(NG);
+    const uint32_t kc = *reinterpret_cast<const uint16_t*>(krec + 64 * r + 16 * (lane % 8 / 2) + 4 * (lane / 8) + 2 * (lane & 1));
+    const uint8_t* src = vrec + 512 * (lane / 16) + 16 * (r % 8 / 2) + 4 * (lane / 4 % 4) + (r / 8) + 2 * (r % 2);
+    uint32_t vc = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vc |= ((uint32_t)src[64 * (4 * (lane & 1) + e)] >> (lane & 2 ? 4 : 0) & 15u) << (4 * e);
+    const uint32_t kw = *reinterpret_cast<const uint32_t*>(krec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r);
+    const uint32_t vw = *reinterpret_cast<const uint32_t*>(vrec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r);
+    float x[4], y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = kv4_scale(kw) * ((float)(kc >> (4 * e) & 15u) + kv4_zero(kw));
+      y[e] = kv4_scale(vw) * ((float)(vc >> (4 * e) & 15u) + kv4_zero(vw));
+    }
+    ko = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    vo = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+  }
+  const size_t at = ((size_t)row * a.heads + head) * HD + 4 * lane;
+  *reinterpret_cast<uint2*>(a.k_out + at) = ko;
+  *reinterpret_cast<uint2*>(a.v_out + at) = vo;
+}
+
+// ------------------------------------------------------------------ page copies
+
+constexpr int CP_TENSORS = 192;   // caches per launch
+constexpr int CP_PAIRS = 512;     // pages per launch
+constexpr int CP_THREADS = 256;
+constexpr int CP_UNITS = 4;       // 16-byte units per thread: a CTA moves 16 KB
+
+// Pages and addresses travel in the launch's arguments: no copy to the device,
+// nothing to keep alive until the kernel has read it.
+struct CopyPagesArgs {
+  uint8_t* base[CP_TENSORS];
+  int2 pair[CP_PAIRS];      // (source, destination)
+  int64_t page_units;       // 16-byte units per page
+  int pairs, chunks;        // chunks: CTAs per page
+};
+
+// grid (chunk + chunks * pair, tensor).
+__global__ void __launch_bounds__(CP_THREADS) copy_pages_kernel(const __grid_constant__ CopyPagesArgs a) {
+  const int p = blockIdx.x / a.chunks;
+  const int64_t u0 = (int64_t)(blockIdx.x - p * a.chunks) * (CP_THREADS * CP_UNITS) + threadIdx.x;
+  uint8_t* base = a.base[blockIdx.y];
+  const uint4* src = reinterpret_cast<const uint4*>(base) + a.pair[p].x * a.page_units;
+  uint4* dst = reinterpret_cast<uint4*>(base) + a.pair[p].y * a.page_units;
+  uint4 v[CP_UNITS];
+#pragma unroll
+  for (int i = 0; i < CP_UNITS; ++i)
+    if (u0 + i * CP_THREADS < a.page_units) v[i] = __ldcs(src + u0 + i * CP_THREADS);
+#pragma unroll
+  for (int i = 0; i < CP_UNITS; ++i)
+    if (u0 + i * CP_THREADS < a.page_units) __stcs(dst + u0 + i * CP_THREADS, v[i]);
+}
+
+}  // namespace dsv
+
+// ---------------------------------------------------------------- bindings
+
+// Checks a 4-bit cache and returns its number of groups per row. (Numbers enter
+// these messages as strings: formatting one through a stream crashed in a process
+// whose CUDA driver was loaded.)
+int dsv_kv4_groups(const torch::Tensor& cache, const char* op) {
+  TORCH_CHECK_VALUE(cache.is_cuda() && cache.scalar_type() == at::kByte && cache.dim() == 5 && cache.size(3) == 2,
+                    op, ": cache must be a CUDA uint8 tensor [pages, kv heads, page size / 16, 2, record bytes]");
+  TORCH_CHECK_VALUE(cache.is_contiguous() && reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, op,
+                    ": cache must be contiguous and 16-byte aligned");
+  const int64_t rec = cache.size(4);
+  const int ng = rec == dsv::kv4_record(1) ? 1 : rec == dsv::kv4_record(2) ? 2 : rec == dsv::kv4_record(4) ? 4 : 0;
+  TORCH_CHECK_VALUE(ng != 0, op, ": record of ", std::to_string(rec), " bytes is none of 1088, 1152, 1280 (groups of 128, 64, 32)");
+  return ng;
+}
+
+static void kv4_rows(const char* op, const torch::Tensor& x, int heads, int64_t rows, int64_t& row, int64_t& head,
+                     bool& vec) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.scalar_type() == at::kBFloat16, op, ": k and v must be bf16 CUDA tensors");
+  const bool flat = x.dim() == 2;
+  TORCH_CHECK_VALUE(flat ? x.size(1) == (int64_t)heads * dsv::HD
+                         : x.dim() == 3 && x.size(1) == heads && x.size(2) == dsv::HD,
+                    op, ": k and v must be [rows, kv heads * 128] or [rows, kv heads, 128]");
+  TORCH_CHECK_VALUE(x.size(0) == rows && x.stride(-1) == 1, op, ": k, v and slots must have the same rows, contiguous along the channels");
+  row = x.stride(0);
+  head = flat ? dsv::HD : x.stride(1);
+  vec = vec && row % 4 == 0 && head % 4 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 8 == 0;
+}
+
+static dsv::Kv4RowsArgs kv4_rows_args(const char* op, const torch::Tensor& cache, const torch::Tensor& slots) {
+  TORCH_CHECK_VALUE(slots.is_cuda() && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                        slots.device() == cache.device(),
+                    op, ": slots must be a contiguous int64 vector on the cache's device");
+  TORCH_CHECK_VALUE(slots.size(0) < (int64_t(1) << 31), op, ": too many rows");
+  dsv::Kv4RowsArgs a{};
+  a.cache = cache.data_ptr<uint8_t>();
+  a.slots = slots.data_ptr<int64_t>();
+  a.rows = (int)slots.size(0);
+  a.heads = (int)cache.size(1);
+  a.page = (int)cache.size(2) * 16;
+  a.num_slots = cache.size(0) * a.page;
+  return a;
+}
+
+void dsv_kv4_write(torch::Tensor k, torch::Tensor v, torch::Tensor cache, torch::Tensor slots) {
+  using namespace dsv;
+  const int ng = dsv_kv4_groups(cache, "kv4_write");
+  Kv4RowsArgs a = kv4_rows_args("kv4_write", cache, slots);
+  bool vec = true;
+  kv4_rows("kv4_write", k, a.heads, a.rows, a.k_row, a.k_head, vec);
+  kv4_rows("kv4_write", v, a.heads, a.rows, a.v_row, a.v_head, vec);
+  TORCH_CHECK_VALUE(k.device() == cache.device() && v.device() == cache.device(),
+                    "kv4_write: k, v and the cache must be on one device");
+  const int64_t blocks = ((int64_t)a.rows * a.heads + 7) / 8;
+  if (blocks == 0) return;
+  a.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
+  c10::cuda::CUDAGuard guard(cache.device());
+  auto kernel = ng == 1 ? kv4_write_kernel<1> : ng == 2 ? kv4_write_kernel<2> : kv4_write_kernel<4>;
+  kernel<<<(unsigned)blocks, 256, 0, at::cuda::getCurrentCUDAStream()>>>(a, vec);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+std::tuple<torch::Tensor, torch::Tensor> dsv_kv4_read(torch::Tensor cache, torch::Tensor slots) {
+  using namespace dsv;
+  const int ng = dsv_kv4_groups(cache, "kv4_read");
+  Kv4RowsArgs a = kv4_rows_args("kv4_read", cache, slots);
+  c10::cuda::CUDAGuard guard(cache.device());
+  auto opt = cache.options().dtype(at::kBFloat16);
+  torch::Tensor k = torch::empty({a.rows, (int64_t)a.heads * HD}, opt), v = torch::empty_like(k);
+  a.k_out = reinterpret_cast<__nv_bfloat16*>(k.data_ptr());
+  a.v_out = reinterpret_cast<__nv_bfloat16*>(v.data_ptr());
+  const int64_t blocks = ((int64_t)a.rows * a.heads + 7) / 8;
+  if (blocks > 0) {
+    auto kernel = ng == 1 ? kv4_read_kernel<1> : ng == 2 ? kv4_read_kernel<2> : kv4_read_kernel<4>;
+    kernel<<<(unsigned)blocks, 256, 0, at::cuda::getCurrentCUDAStream()>>>(a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return {k, v};
+}
+
+// Returns the number of kernels launched.
+int64_t dsv_copy_pages(std::vector<torch::Tensor> caches, std::vector<int64_t> src, std::vector<int64_t> dst) {
+  using namespace dsv;
+  if (caches.empty() || src.empty()) return 0;
+  const torch::Tensor& c0 = caches[0];
+  const int64_t pages = c0.size(0);
+  const int64_t bytes = pages > 0 ? (int64_t)c0.nbytes() / pages : 0;
+  for (const auto& c : caches) {
+    TORCH_CHECK_VALUE(c.is_cuda() && c.device() == c0.device() && c.is_contiguous() && c.dim() >= 1 &&
+                          c.size(0) == pages && (int64_t)c.nbytes() == pages * bytes,
+                      "copy_pages: caches must be contiguous tensors of one shape and element size on one device");
+    TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0,
+                      "copy_pages: caches must be 16-byte aligned");
+  }
+  TORCH_CHECK_VALUE(bytes % 16 == 0, "copy_pages: a page must be a multiple of 16 bytes");
+  if (bytes == 0) return 0;
+  c10::cuda::CUDAGuard guard(c0.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  CopyPagesArgs a;
+  a.page_units = bytes / 16;
+  const int64_t chunks = (a.page_units + CP_THREADS * CP_UNITS - 1) / (CP_THREADS * CP_UNITS);
+  TORCH_CHECK_VALUE(chunks * CP_PAIRS < (int64_t(1) << 31), "copy_pages: page too large");
+  a.chunks = (int)chunks;
+  int64_t launches = 0;
+  for (size_t t0 = 0; t0 < caches.size(); t0 += CP_TENSORS) {
+    const int nt = (int)std::min<size_t>(CP_TENSORS, caches.size() - t0);
+    for (int i = 0; i < nt; ++i) a.base[i] = reinterpret_cast<uint8_t*>(caches[t0 + i].data_ptr());
+    for (size_t p0 = 0; p0 < src.size(); p0 += CP_PAIRS) {
+      a.pairs = (int)std::min<size_t>(CP_PAIRS, src.size() - p0);
+      for (int i = 0; i < a.pairs; ++i) a.pair[i] = make_int2((int)src[p0 + i], (int)dst[p0 + i]);
+      copy_pages_kernel<<<dim3((unsigned)(a.pairs * a.chunks), (unsigned)nt), CP_THREADS, 0, stream>>>(a);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+      ++launches;
+    }
+  }
+  return launches;
+}
+
+DSV_ERROR_ACCESSOR(dsv_read_error_kv4_cache)

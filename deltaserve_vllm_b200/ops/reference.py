@@ -149,6 +149,128 @@ def paged_decode(q, k_cache, v_cache, block_tables, ctx_lens, out, num_heads, sc
     return paged_prefill(q, k_cache, v_cache, block_tables, cu, ctx_lens, out, num_heads, scale)
 
 
+# ----------------------------------------------------------------- 4-bit KV cache
+# (format and code order: csrc/kv4.cuh)
+
+KV4_LIMIT = 8192.0
+KV4_TINY = 2.0 ** -120
+
+
+def _kv4_group(cache) -> int:
+    if cache.dtype != torch.uint8 or cache.dim() != 5 or cache.shape[3] != 2:
+        raise ValueError("kv4 cache must be uint8 [pages, kv heads, page size / 16, 2, record bytes]")
+    for group in (32, 64, 128):
+        if cache.shape[4] == 1024 + 64 * (128 // group):
+            return group
+    raise ValueError(f"record of {cache.shape[4]} bytes is none of 1088, 1152, 1280 (groups of 128, 64, 32)")
+
+
+def kv4_places(device) -> tuple[torch.Tensor, torch.Tensor]:
+    """(byte, shift) in its record of the code of every (K or V, token, channel): int64 [2, 16, 128]."""
+    tok = torch.arange(16, device=device)[:, None]
+    ch = torch.arange(128, device=device)[None]
+    k_nibble = 128 * tok + 32 * (ch // 8 % 4) + 8 * (ch // 32) + ch % 8
+    word = 128 * (ch // 64) + 4 * (4 * (ch % 8) + tok % 8 // 2) + ch // 16 % 4
+    v_nibble = 8 * word + ch // 8 % 2 + 2 * (tok // 8) + 4 * (tok % 2)
+    nib = torch.stack([k_nibble, v_nibble])
+    return nib // 2, nib % 2 * 4
+
+
+def kv4_quantise(x, group):
+    """Codes uint8 [..., 128] and (scale, zero point) fp32 [..., 128 / group] of rows ``x``."""
+    x = torch.nan_to_num(x.float(), nan=0.0, posinf=KV4_LIMIT, neginf=-KV4_LIMIT).clamp(-KV4_LIMIT, KV4_LIMIT)
+    x = x.unflatten(-1, (-1, group))
+    lo, hi = x.amin(-1).clamp(max=0.0), x.amax(-1).clamp(min=0.0)
+    scale = ((hi - lo) / 15.0).to(torch.bfloat16).float()
+    scale[scale < KV4_TINY] = 0.0
+    inv = torch.where(scale > 0, 1.0 / scale, torch.zeros_like(scale))
+    zero = (lo * inv).half().float()
+    codes = torch.round(x * inv[..., None] - zero[..., None]).clamp(0, 15).to(torch.uint8)
+    return codes.flatten(-2), scale, zero
+
+
+def _kv4_at(cache, slots):
+    """Index tensors (page, sub, token) of non-negative slots."""
+    page = cache.shape[2] * 16
+    return slots // page, slots % page // 16, slots % 16
+
+
+def kv4_write(k, v, cache, slots):
+    group, hkv = _kv4_group(cache), cache.shape[1]
+    if slots.dtype != torch.int64 or slots.dim() != 1 or len(slots) != k.shape[0] or len(slots) != v.shape[0]:
+        raise ValueError("kv4_write: slots must be an int64 vector with one slot per row of k and v")
+    if any(x[0].numel() != hkv * 128 for x in (k, v) if len(x)):
+        raise ValueError("kv4_write: k and v must be [rows, kv heads * 128] or [rows, kv heads, 128]")
+    byte, shift = kv4_places(cache.device)
+    for i, slot in enumerate(slots.tolist()):
+        if slot < 0:
+            continue
+        page, sub, tok = (int(x) for x in _kv4_at(cache, torch.tensor(slot)))
+        for which, x in enumerate((k[i], v[i])):
+            codes, scale, zero = kv4_quantise(x.reshape(hkv, 128), group)
+            rec = cache[page, :, sub, which]
+            b, s = byte[which, tok], shift[which, tok]
+            row = torch.zeros_like(rec).scatter_add_(1, b.expand(hkv, -1), codes << s.to(torch.uint8))
+            rec[:, b] = row[:, b]
+            words = torch.stack([zero.half().view(torch.int16), scale.to(torch.bfloat16).view(torch.int16)], -1)
+            rec[:, 1024:].view(hkv, -1, 16, 4)[:, :, tok] = words.view(torch.uint8)
+
+
+def kv4_values(cache):
+    """fp32 [..., 2, 16, 128]: what the records of a cache (or of some pages of it) stand for."""
+    group = {1280: 32, 1152: 64, 1088: 128}[cache.shape[-1]]
+    byte, shift = kv4_places(cache.device)
+    at = byte.flatten(1).expand(*cache.shape[:-1], -1)
+    codes = cache.gather(-1, at) >> shift.flatten(1).to(torch.uint8) & 15
+    word = cache[..., 1024:].contiguous().view(torch.int16).unflatten(-1, (-1, 16, 2)).transpose(-3, -2)
+    zero = word[..., 0].contiguous().view(torch.float16).float()[..., None]
+    scale = word[..., 1].contiguous().view(torch.bfloat16).float()[..., None]
+    return (scale * (codes.unflatten(-1, (16, -1, group)).float() + zero)).flatten(-2)
+
+
+def kv4_read(cache, slots):
+    _kv4_group(cache)
+    if slots.dtype != torch.int64 or slots.dim() != 1:
+        raise ValueError("kv4_read: slots must be an int64 vector")
+    page, sub, tok = _kv4_at(cache, slots.clamp(min=0))
+    kv = kv4_values(cache[page, :, sub])[torch.arange(len(slots), device=slots.device), :, :, tok]   # [T, H, 2, 128]
+    kv = torch.where((slots >= 0)[:, None, None, None], kv, torch.zeros_like(kv)).to(torch.bfloat16)
+    return kv[:, :, 0].flatten(1), kv[:, :, 1].flatten(1)
+
+
+def _kv4_pages(cache, block_table, ctx):
+    """One sequence's K and V pages as fp32 caches of the bf16 layout."""
+    need = -(-ctx // (cache.shape[2] * 16))
+    kv = kv4_values(cache[block_table[:need].long()])                                  # [P, H, sub, 2, 16, 128]
+    return kv[:, :, :, 0].flatten(2, 3), kv[:, :, :, 1].flatten(2, 3)
+
+
+def paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale):
+    _kv4_group(cache)
+    if num_heads % cache.shape[1]:
+        raise ValueError("query heads must be a multiple of the kv heads")
+    for s in range(ctx_lens.shape[0]):
+        q0, q1, ctx = int(cu_q[s]), int(cu_q[s + 1]), int(ctx_lens[s])
+        if ctx == 0:
+            out[q0:q1] = 0
+            continue
+        k, v = _kv4_pages(cache, block_tables[s], ctx)
+        one = torch.arange(k.shape[0], device=cache.device, dtype=torch.int32)[None]
+        paged_prefill(q[q0:q1], k, v, one, torch.tensor([0, q1 - q0]), ctx_lens[s:s + 1], out[q0:q1], num_heads, scale)
+    return out
+
+
+def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale):
+    cu = torch.arange(ctx_lens.shape[0] + 1, dtype=torch.int32)
+    return paged_prefill4(q, cache, block_tables, cu, ctx_lens, out, num_heads, scale)
+
+
+def copy_pages(caches, src, dst):
+    src, dst = torch.as_tensor(src), torch.as_tensor(dst)
+    for c in caches:
+        c[dst.to(c.device)] = c[src.to(c.device)]
+
+
 def lora_shrink(x, A, slot_ids, Z, seg):
     slots, PR, K = A.shape
     Z.zero_()

@@ -1,0 +1,342 @@
+"""The 4-bit KV cache's kernels: write / read bit for bit, decode attention
+against 64-bit arithmetic on the values the codes stand for, page copies."""
+import pytest
+import torch
+
+from deltaserve_vllm_b200 import ops
+from deltaserve_vllm_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SCALE = 128 ** -0.5
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    yield
+    assert ops.check_device_error() == 0
+
+
+@pytest.fixture(scope="module")
+def ws():
+    return ops.kv4_workspace(DEV)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rows(g, *shape, wide=6.0):
+    x = torch.randn(*shape, 128, generator=g, device=DEV)
+    return (x * torch.where(torch.rand(128, generator=g, device=DEV) < 0.05, wide, 1.0)).to(torch.bfloat16)
+
+
+def empty_cache(pages, hkv, page, group):
+    """A cache of 0xff bytes: an unwritten scale or zero point is a NaN."""
+    return torch.full(ops.kv4_cache_shape(pages, hkv, page, group), 255, dtype=torch.uint8, device=DEV)
+
+
+def special_rows(g, n, hkv):
+    """Rows with everything a group can hold: zeros, one sign, one value, tiny, huge, infinities, NaN."""
+    x = rows(g, n, hkv)
+    x[0::8] = 0
+    x[1::8] = x[1::8].abs() + 3
+    x[2::8] = -2.5
+    x[3::8] *= 2.0 ** -130
+    x[4::8] *= 3e4
+    x[5::8, :, ::17] = float("inf")
+    x[6::8, :, 1::29] = float("nan")
+    x[7::8, :, 5] = float("-inf")
+    return x
+
+
+@pytest.mark.parametrize("group", ops.KV4_GROUPS)
+@pytest.mark.parametrize("n,hkv,page", [(1, 1, 16), (16, 2, 16), (37, 3, 48), (300, 8, 64), (129, 1, 128)])
+@pytest.mark.parametrize("start", [0, 5])
+def test_write_and_read_match_the_format(n, hkv, page, group, start):
+    g = gen(n + page + group)
+    k, v = special_rows(g, n, hkv), special_rows(g, n, hkv)
+    pages = -(-(start + n) // page) + 2
+    perm = torch.randperm(pages, generator=g, device=DEV)
+    pos = start + torch.arange(n, device=DEV)
+    slots = perm[pos // page] * page + pos % page
+    if n > 20:
+        slots[3::7] = -1
+    got = empty_cache(pages, hkv, page, group)
+    exp = got.clone().cpu()
+    ops.kv4_write(k.flatten(1), v.flatten(1), got, slots)
+    ref.kv4_write(k.flatten(1).cpu(), v.flatten(1).cpu(), exp, slots.cpu())
+    assert torch.equal(got.cpu(), exp)
+    gk, gv = ops.kv4_read(got, slots)
+    ek, ev = ref.kv4_read(exp, slots.cpu())
+    assert torch.equal(gk.cpu(), ek) and torch.equal(gv.cpu(), ev)
+
+
+@pytest.mark.parametrize("order", ["shuffled", "reversed", "two_runs"])
+def test_write_takes_slots_in_any_order(order):
+    """Slots that do not follow one another, or do so only for a part of a 16-token record."""
+    g = gen(3)
+    n, hkv, page, group = 96, 2, 64, 64
+    k, v = rows(g, n, hkv), rows(g, n, hkv)
+    slots = {"shuffled": torch.randperm(256, generator=g, device=DEV)[:n],
+             "reversed": torch.arange(n - 1, -1, -1, device=DEV) + 64,
+             "two_runs": torch.cat([torch.arange(8, device=DEV) + 64, torch.arange(n - 8, device=DEV) + 136])}[order]
+    got = empty_cache(4, hkv, page, group)
+    exp = got.clone().cpu()
+    ops.kv4_write(k.flatten(1), v.flatten(1), got, slots)
+    ref.kv4_write(k.flatten(1).cpu(), v.flatten(1).cpu(), exp, slots.cpu())
+    assert torch.equal(got.cpu(), exp)
+
+
+@pytest.mark.parametrize("layout", ["qkv", "heads", "odd"])
+def test_write_takes_strided_rows(layout):
+    g = gen(5)
+    n, hkv, page, group = 50, 2, 16, 32
+    slots = torch.arange(n, device=DEV)
+    base = rows(g, n, 9).flatten(1)
+    if layout == "qkv":           # column blocks of a fused projection
+        k, v = base[:, 128:384], base[:, 640:896]
+    elif layout == "heads":       # [rows, heads, 128] with its own head stride
+        k, v = base.view(n, 9, 128)[:, 1:8:4], base.view(n, 9, 128)[:, 2:9:4]
+    else:                         # rows that start at an odd element
+        k, v = base[:, 1:257], base[:, 259:515]
+    got = empty_cache(4, hkv, page, group)
+    exp = got.clone().cpu()
+    ops.kv4_write(k, v, got, slots)
+    ref.kv4_write(k.cpu(), v.cpu(), exp, slots.cpu())
+    assert torch.equal(got.cpu(), exp)
+
+
+def test_write_outside_the_cache_is_an_error_not_a_write():
+    g = gen(6)
+    k = rows(g, 2, 1)
+    cache = empty_cache(2, 1, 16, 64)
+    before = cache.clone()
+    ops.kv4_write(k.flatten(1), k.flatten(1), cache, torch.tensor([32, 1 << 40], device=DEV))
+    assert torch.equal(cache, before)
+    assert ops.check_device_error() != 0
+
+
+def filled(g, contexts, hkv, page, group, extra_cols=2):
+    """A cache of quantised rows for every context, its block tables (unused
+    entries out of range) and the values: float64 [n][2][hkv, ctx, 128]."""
+    need = [-(-c // page) for c in contexts]
+    pages = sum(need) + 1
+    perm = torch.randperm(pages, generator=g, device=DEV).tolist()
+    tables = torch.full((len(contexts), max(need) + extra_cols), 1 << 30, dtype=torch.int32)
+    cache = empty_cache(pages, hkv, page, group)
+    values = []
+    for i, c in enumerate(contexts):
+        mine = [perm.pop() for _ in range(need[i])]
+        tables[i, :need[i]] = torch.tensor(mine, dtype=torch.int32)
+        slots = torch.tensor([mine[p // page] * page + p % page for p in range(c)], dtype=torch.int64, device=DEV)
+        if c:
+            ops.kv4_write(rows(g, c, hkv).flatten(1), (rows(g, c, hkv) * 0.5).flatten(1), cache, slots)
+        rec = ref.kv4_values(cache[torch.tensor(mine, device=DEV, dtype=torch.long)]).double()
+        values.append([rec[:, :, :, w].permute(1, 0, 2, 3, 4).reshape(hkv, -1, 128)[:, :c] for w in (0, 1)])
+    return cache, tables.to(DEV), values
+
+
+def attention64(q, k, v, seen):
+    """float64 softmax attention: q [m, heads, 128], k / v [hkv, ctx, 128], seen [m, ctx]."""
+    q = q.double().unflatten(1, (k.shape[0], -1))
+    s = torch.einsum("mhgd,hkd->mhgk", q, k) * SCALE
+    s = s.masked_fill(~seen[:, None, None], float("-inf"))
+    return torch.einsum("mhgk,hkd->mhgd", torch.softmax(s, -1), v).flatten(1)
+
+
+def check(got, exp, v):
+    """bf16 rounding of the result (2^-9, taken twice for values next to a
+    rounding step) and, absolute: weights in 11 bits against codes of up to twice
+    the largest value (2^-10), and scores summed in fp32 (below 2^-11 of a weight
+    for these inputs, moving an average of values by at most twice that)."""
+    assert got.shape == exp.shape
+    top = float(v.abs().max()) if v.numel() else 0.0
+    err = (got.double() - exp).abs()
+    assert bool((err <= exp.abs() * 2 ** -8 + top * 2 ** -9).all()), float((err - exp.abs() * 2 ** -8).max() / top)
+
+
+def check_decode(contexts, heads, hkv, page, group, ws, seed=0, q=None):
+    g = gen(seed + page + group + heads)
+    cache, tables, values = filled(g, contexts, hkv, page, group)
+    ctx = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    if q is None:
+        q = torch.randn(len(contexts), (heads + 2) * 128, generator=g, device=DEV).to(torch.bfloat16)[:, 128:-128]
+    out = torch.full((len(contexts), heads * 128 + 8), float("nan"), dtype=torch.bfloat16, device=DEV)[:, :heads * 128]
+    ops.paged_decode4(q, cache, tables, ctx, out, heads, SCALE, ws)
+    again = torch.empty_like(out)
+    ops.paged_decode4(q, cache, tables, ctx, again, heads, SCALE, ws)
+    assert torch.equal(out, again)
+    for i, c in enumerate(contexts):
+        if c == 0:
+            assert bool((out[i] == 0).all())
+            continue
+        exp = attention64(q[i].view(1, heads, 128), *values[i], torch.ones(1, c, dtype=torch.bool, device=DEV))
+        check(out[i:i + 1], exp, values[i][1])
+    return out
+
+
+@pytest.mark.parametrize("group", ops.KV4_GROUPS)
+@pytest.mark.parametrize("page", [16, 48, 64, 128])
+def test_decode_ragged(page, group, ws):
+    check_decode([0, 1, 15, 16, 17, 63, 64, 65, 127, 300, 0, 1000], 8, 2, page, group, ws)
+
+
+@pytest.mark.parametrize("per", list(range(1, 17)))
+def test_decode_query_heads_per_kv_head(per, ws):
+    check_decode([77, 1, 512, 33], 2 * per, 2, 64, 64 if per % 2 else 32, ws)
+
+
+@pytest.mark.parametrize("batch,ctx", [(1, 1), (1, 5000), (3, 2049), (130, 65), (700, 20)])
+def test_decode_batches(batch, ctx, ws):
+    check_decode([max(1, ctx - i % 19) for i in range(batch)], 4, 1, 16, 128, ws)
+
+
+def test_decode_sharp_and_flat_scores(ws):
+    """Scores far apart (one key takes everything, later keys raise the maximum) and all equal."""
+    g = gen(9)
+    q = torch.randn(2, 4 * 128, generator=g, device=DEV)
+    q[0] *= 40
+    q[1] = 0
+    check_decode([700, 700], 4, 2, 64, 64, ws, q=q.to(torch.bfloat16))
+
+
+def test_decode_query_magnitudes(ws):
+    """The query is scaled by a power of two on its way to 16 bits: none overflows or vanishes."""
+    g = gen(10)
+    q = torch.randn(4, 4 * 128, generator=g, device=DEV) * torch.tensor([1e-30, 1e-4, 1.0, 100.0], device=DEV)[:, None]
+    q[2, ::7] *= 1e-4
+    check_decode([100, 100, 100, 100], 4, 1, 16, 64, ws, q=q.to(torch.bfloat16))
+
+
+def test_decode_nan_query_stays_in_its_head(ws):
+    g = gen(11)
+    cache, tables, values = filled(g, [50], 2, 16, 64)
+    q = torch.randn(1, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    q[0, 130] = float("nan")
+    out = torch.empty_like(q)
+    ops.paged_decode4(q, cache, tables, torch.tensor([50], dtype=torch.int32, device=DEV), out, 4, SCALE, ws)
+    assert bool(out[0, 128:256].isnan().all())
+    assert bool(out[0, :128].isfinite().all()) and bool(out[0, 256:].isfinite().all())
+
+
+def test_decode_on_another_stream_and_in_a_graph(ws):
+    """The call goes to the current stream, and a captured call follows new lengths and tables."""
+    g = gen(12)
+    cache, tables, values = filled(g, [400, 90], 2, 64, 64)
+    ctx = torch.tensor([400, 90], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 8 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    exp = ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, ws)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.paged_decode4(q, cache, tables, ctx, out, 8, SCALE, ws)
+    side.synchronize()
+    assert torch.equal(out, exp)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_decode4(q, cache, tables, ctx, out, 8, SCALE, ws)
+    ctx.copy_(torch.tensor([13, 65], dtype=torch.int32))
+    graph.replay()
+    exp = ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, ws)
+    torch.cuda.synchronize()
+    assert torch.equal(out, exp)
+    check(out[:1], attention64(q[0].view(1, 8, 128), values[0][0][:, :13], values[0][1][:, :13],
+                               torch.ones(1, 13, dtype=torch.bool, device=DEV)), values[0][1])
+
+
+def test_offsets_past_32_bits(ws):
+    """A cache of over 4 GiB: pages at its end are written, read, attended and copied."""
+    g = gen(13)
+    hkv, page, group = 8, 128, 64
+    pages = (1 << 32) // (hkv * page * 144) + 40
+    cache = torch.zeros(ops.kv4_cache_shape(pages, hkv, page, group), dtype=torch.uint8, device=DEV)
+    assert cache.numel() > 1 << 32
+    n, last = 200, [pages - 1, pages - 7]
+    k, v = rows(g, n, hkv).flatten(1), rows(g, n, hkv).flatten(1)
+    pos = torch.arange(n, device=DEV)
+    slots = torch.tensor(last, device=DEV)[pos // page] * page + pos % page
+    ops.kv4_write(k, v, cache, slots)
+    small = torch.zeros(ops.kv4_cache_shape(2, hkv, page, group), dtype=torch.uint8, device=DEV)
+    ops.kv4_write(k, v, small, pos)
+    assert torch.equal(cache[last], small)
+    assert torch.equal(ops.kv4_read(cache, slots)[1], ops.kv4_read(small, pos)[1])
+    q = torch.randn(1, 16 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    ctx = torch.tensor([n], dtype=torch.int32, device=DEV)
+    a = ops.paged_decode4(q, cache, torch.tensor([last], dtype=torch.int32, device=DEV), ctx, torch.empty_like(q), 16,
+                          SCALE, ws)
+    b = ops.paged_decode4(q, small, torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), ctx, torch.empty_like(q), 16,
+                          SCALE, ws)
+    assert torch.equal(a, b)
+    ops.copy_pages([cache], last, [pages - 2, 3])
+    assert torch.equal(cache[[pages - 2, 3]], small)
+
+
+def test_decode_page_outside_the_cache_is_an_error(ws):
+    g = gen(14)
+    cache, tables, _ = filled(g, [40], 1, 16, 64)
+    tables[0, 1] = 1 << 20
+    q = torch.randn(1, 128, generator=g, device=DEV).to(torch.bfloat16)
+    ops.paged_decode4(q, cache, tables, torch.tensor([40], dtype=torch.int32, device=DEV), torch.empty_like(q), 1,
+                      SCALE, ws)
+    assert ops.check_device_error() != 0
+
+
+@pytest.mark.parametrize("kind", ["int4", "bf16", "bytes16"])
+@pytest.mark.parametrize("layers,pages,moves", [(1, 2, 1), (3, 40, 20), (200, 9, 3), (2, 1300, 600)])
+def test_copy_pages(kind, layers, pages, moves):
+    g = gen(layers + pages)
+    shape = {"int4": ops.kv4_cache_shape(pages, 2, 16, 64), "bf16": (pages, 2, 16, 128), "bytes16": (pages, 16)}[kind]
+    caches = [torch.randint(0, 256, shape, generator=g, device=DEV, dtype=torch.uint8) for _ in range(layers)]
+    if kind == "bf16":
+        caches = [c.to(torch.bfloat16) for c in caches]
+    exp = [c.clone() for c in caches]
+    perm = torch.randperm(pages, generator=g, device=DEV).tolist()
+    src, dst = perm[:moves], perm[moves:2 * moves]
+    src[-1] = src[0]                       # one page may be copied to several
+    ops.copy_pages(caches, src, dst)
+    ref.copy_pages(exp, src, dst)
+    assert all(torch.equal(a, b) for a, b in zip(caches, exp))
+
+
+# ----------------------------------------------------------------- refusals
+
+def test_refusals(ws):
+    cache = empty_cache(4, 2, 16, 64)
+    k = torch.zeros(3, 256, dtype=torch.bfloat16, device=DEV)
+    slots = torch.arange(3, device=DEV)
+    for bad in (dict(cache=cache[..., :1100].contiguous()), dict(cache=cache.view(torch.int8)), dict(cache=cache[:, :1]),
+                dict(k=k.float()), dict(k=k[:, :128]), dict(k=k[:2]), dict(k=k.cpu()), dict(slots=slots.int()),
+                dict(slots=slots[:2]), dict(slots=slots.cpu()), dict(k=torch.zeros(256, 3, dtype=torch.bfloat16, device=DEV).t())):
+        a = dict(dict(cache=cache, k=k, slots=slots), **bad)
+        with pytest.raises(ValueError):
+            ops.kv4_write(a["k"], k, a["cache"], a["slots"])
+    with pytest.raises(ValueError):
+        ops.kv4_read(cache, slots.int())
+    q = torch.zeros(2, 4 * 128, dtype=torch.bfloat16, device=DEV)
+    tables = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    ctx = torch.ones(2, dtype=torch.int32, device=DEV)
+    good = dict(q=q, cache=cache, tables=tables, ctx=ctx, out=torch.empty_like(q), heads=4, ws=ws)
+    ops.paged_decode4(q, cache, tables, ctx, good["out"], 4, SCALE, ws)
+    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(heads=3), dict(heads=0), dict(heads=8), dict(tables=tables.long()),
+                dict(tables=tables[:1]), dict(ctx=ctx.long()), dict(ctx=ctx[:1]), dict(ws=ws[:100]), dict(out=q.float()),
+                dict(out=q.cpu()), dict(ctx=ctx.cpu()), dict(q=torch.zeros(2, 4 * 128 + 4, dtype=torch.bfloat16, device=DEV)[:, 4:])):
+        a = dict(good, **bad)
+        with pytest.raises(ValueError):
+            ops.paged_decode4(a["q"], a["cache"], a["tables"], a["ctx"], a["out"], a["heads"], SCALE, a["ws"])
+    wide = torch.zeros(2, 34 * 128, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError):
+        ops.paged_decode4(wide, cache, tables, ctx, torch.empty_like(wide), 34, SCALE, ws)
+
+
+def test_copy_refusals():
+    caches = [empty_cache(4, 1, 16, 64) for _ in range(2)]
+    for src, dst in (([0], [1, 2]), ([0], [4]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [0])):
+        with pytest.raises(ValueError):
+            ops.copy_pages(caches, src, dst)
+    with pytest.raises(ValueError):
+        ops.copy_pages([caches[0], empty_cache(5, 1, 16, 64)], [0], [1])
+    with pytest.raises(ValueError):
+        ops.copy_pages([torch.zeros(4, 10, dtype=torch.uint8, device=DEV)], [0], [1])
+    ops.copy_pages(caches, [], [])
