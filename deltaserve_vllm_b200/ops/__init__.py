@@ -294,7 +294,14 @@ def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws):
 
 
 def paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale, ws):
-    """:func:`paged_prefill` over a 4-bit cache."""
+    """:func:`paged_prefill` over a 4-bit cache: the new tokens of packed
+    sequences (``cu_q`` int32 ``[S + 1]``: their offsets in ``q`` / ``out``, bf16
+    ``[T, Hq * 128]`` with 16-byte aligned rows) against ``ctx_lens`` cached
+    tokens each, the new ones among them and last. Tiles are found on the device:
+    no tile list. ``ws`` from :func:`kv4_workspace`."""
+    if cache.is_cuda:
+        LAUNCHES[0] += _native(0).paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale, ws)
+        return out
     return ref.paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale)
 
 

@@ -51,6 +51,8 @@ int64_t dsv_copy_pages(std::vector<torch::Tensor> caches, std::vector<int64_t> s
 int64_t dsv_kv4_workspace_bytes();
 int64_t dsv_paged_decode4(torch::Tensor q, torch::Tensor cache, torch::Tensor tables, torch::Tensor ctx,
                           torch::Tensor out, int64_t heads, double scale, torch::Tensor ws);
+int64_t dsv_paged_prefill4(torch::Tensor q, torch::Tensor cache, torch::Tensor tables, torch::Tensor cu_q,
+                           torch::Tensor ctx, torch::Tensor out, int64_t heads, double scale, torch::Tensor ws);
 int64_t dsv_read_error_gemm(bool clear);
 int64_t dsv_read_error_attn_bwd(bool clear);
 int64_t dsv_read_error_tp_bwd(bool clear);
@@ -58,10 +60,12 @@ int64_t dsv_read_error_attn_tc(bool clear);
 int64_t dsv_read_error_attn_bwd_tc(bool clear);
 int64_t dsv_read_error_kv4_cache(bool clear);
 int64_t dsv_read_error_kv4_decode(bool clear);
+int64_t dsv_read_error_kv4_prefill(bool clear);
 static int64_t dsv_read_error(bool clear) {
   const int64_t codes[] = {dsv_read_error_gemm(clear), dsv_read_error_attn_bwd(clear), dsv_read_error_tp_bwd(clear),
                            dsv_read_error_attn_tc(clear), dsv_read_error_attn_bwd_tc(clear),
-                           dsv_read_error_kv4_cache(clear), dsv_read_error_kv4_decode(clear)};
+                           dsv_read_error_kv4_cache(clear), dsv_read_error_kv4_decode(clear),
+                           dsv_read_error_kv4_prefill(clear)};
   for (int64_t c : codes)
     if (c != 0) return c;
   return 0;
@@ -158,6 +162,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("copy_pages", &dsv_copy_pages, "copy pages of every layer's cache; returns the launches");
   m.def("kv4_workspace_bytes", &dsv_kv4_workspace_bytes, "bytes of the attention workspace of the 4-bit cache");
   m.def("paged_decode4", &dsv_paged_decode4, "decode attention over a 4-bit paged cache; returns the launches");
+  m.def("paged_prefill4", &dsv_paged_prefill4, "causal attention of new tokens over a 4-bit paged cache; returns the launches");
   m.def("attn_bwd", &dsv_attn_bwd, "varlen causal GQA attention backward (dQ, dK, dV)");
   m.def("attn_fwd_dense", &dsv_attn_fwd_dense, "varlen causal GQA attention forward on packed rows");
   m.def("rms_norm", &dsv_rms_norm, "RMSNorm / fused residual add + RMSNorm (+ row capture)");

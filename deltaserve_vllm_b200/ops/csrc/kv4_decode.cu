@@ -129,6 +129,7 @@ int64_t dsv_paged_decode4(torch::Tensor q, torch::Tensor cache, torch::Tensor ta
   const int64_t B = q.size(0), hkv = cache.size(1);
   TORCH_CHECK_VALUE(heads > 0 && heads % hkv == 0 && heads / hkv <= 16,
                     "paged_decode4: query heads must be 1 to 16 times the kv heads");
+  TORCH_CHECK_VALUE(scale > 0, "paged_decode4: scale must be positive");
   for (const auto* x : {&q, &out})
     TORCH_CHECK_VALUE(x->is_cuda() && x->device() == cache.device() && x->scalar_type() == at::kBFloat16 &&
                           x->dim() == 2 && x->size(0) == B && x->size(1) == heads * HD && x->stride(1) == 1,

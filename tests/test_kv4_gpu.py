@@ -269,6 +269,13 @@ def test_offsets_past_32_bits(ws):
     b = ops.paged_decode4(q, small, torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), ctx, torch.empty_like(q), 16,
                           SCALE, ws)
     assert torch.equal(a, b)
+    q = q.expand(n, -1).contiguous()
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    a = ops.paged_prefill4(q, cache, torch.tensor([last], dtype=torch.int32, device=DEV), cu, ctx, torch.empty_like(q),
+                           16, SCALE, ws)
+    b = ops.paged_prefill4(q, small, torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), cu, ctx,
+                           torch.empty_like(q), 16, SCALE, ws)
+    assert torch.equal(a, b)
     ops.copy_pages([cache], last, [pages - 2, 3])
     assert torch.equal(cache[[pages - 2, 3]], small)
 
@@ -280,6 +287,130 @@ def test_decode_page_outside_the_cache_is_an_error(ws):
     q = torch.randn(1, 128, generator=g, device=DEV).to(torch.bfloat16)
     ops.paged_decode4(q, cache, tables, torch.tensor([40], dtype=torch.int32, device=DEV), torch.empty_like(q), 1,
                       SCALE, ws)
+    assert ops.check_device_error() != 0
+
+
+def check_prefill(new, old, heads, hkv, page, group, ws, seed=0, q=None):
+    """Packed sequences of ``new`` tokens after ``old`` cached ones.
+
+    Besides :func:`check`'s terms the operands are rounded to 11 bits: a value's
+    base (scale x zero point, up to twice the largest value, one rounding for a
+    whole group) moves a score by about 0.005 for these inputs, three times that
+    at worst over half of the value range: 2^-7 of it. Over a whole result the
+    differences average out to below half a bf16 step (2^-8)."""
+    g = gen(seed + page + group + heads)
+    contexts = [a + b for a, b in zip(new, old)]
+    cache, tables, values = filled(g, contexts, hkv, page, group)
+    ctx = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0] + new, device=DEV).cumsum(0).to(torch.int32)
+    total = sum(new)
+    if q is None:
+        q = torch.randn(total, (heads + 2) * 128, generator=g, device=DEV).to(torch.bfloat16)[:, 128:-128]
+    out = torch.full((total, heads * 128 + 8), float("nan"), dtype=torch.bfloat16, device=DEV)[:, :heads * 128]
+    ops.paged_prefill4(q, cache, tables, cu, ctx, out, heads, SCALE, ws)
+    again = torch.empty_like(out)
+    ops.paged_prefill4(q, cache, tables, cu, ctx, again, heads, SCALE, ws)
+    assert torch.equal(out, again)
+    at = 0
+    for i, n in enumerate(new):
+        key = torch.arange(contexts[i], device=DEV)
+        seen = key[None] <= old[i] + torch.arange(n, device=DEV)[:, None]
+        if n == 0:
+            continue
+        exp = attention64(q[at:at + n].reshape(n, heads, 128), *values[i], seen)
+        got = out[at:at + n].double()
+        top = float(values[i][1].abs().max())
+        err = (got - exp).abs()
+        assert bool((err <= exp.abs() * 2 ** -8 + top * 2 ** -7).all()), float(err.max() / top)
+        assert float(err.norm() / exp.norm()) <= 2 ** -8
+        at += n
+    return out
+
+
+@pytest.mark.parametrize("group", ops.KV4_GROUPS)
+@pytest.mark.parametrize("page", [16, 48, 64, 128, 256])
+def test_prefill_ragged(page, group, ws):
+    check_prefill([1, 2, 0, 31, 32, 33, 64, 65, 100, 0, 7], [0, 5, 9, 0, 127, 128, 300, 0, 17, 0, 250], 8, 2, page,
+                  group, ws)
+
+
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 255, 256, 257, 511, 700])
+@pytest.mark.parametrize("old", [0, 1, 128])
+def test_prefill_lengths(n, old, ws):
+    check_prefill([n], [old], 2, 2, 64, 64, ws)
+
+
+@pytest.mark.parametrize("per", list(range(1, 17)))
+def test_prefill_query_heads_per_kv_head(per, ws):
+    check_prefill([75, 1, 140], [11, 40, 0], 2 * per, 2, 64, 64 if per % 2 else 32, ws)
+
+
+def test_prefill_both_tile_widths(ws):
+    """Enough rows for two tiles per CTA, and the same rows in calls that take one."""
+    g = gen(20)
+    new, old = [1200, 300, 900], [100, 0, 33]
+    q = torch.randn(sum(new), 16 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    check_prefill(new, old, 16, 8, 64, 64, ws, q=q)
+
+
+def test_prefill_many_short_sequences(ws):
+    check_prefill([1 + i % 5 for i in range(90)], [i % 41 for i in range(90)], 4, 2, 16, 64, ws)
+
+
+def test_prefill_sharp_and_flat_scores(ws):
+    g = gen(21)
+    q = torch.randn(300, 4 * 128, generator=g, device=DEV)
+    q[::2] *= 40
+    q[1::4] = 0
+    q[5] *= 1e-30
+    q[7] *= 1e4
+    # a score of a query 40 (10^4) times as long moves 40 times as much: only the flat rows are checked as tightly
+    cache, tables, values = filled(g, [300], 2, 64, 64)
+    ctx = torch.tensor([300], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    q = q.to(torch.bfloat16)
+    out = ops.paged_prefill4(q, cache, tables, cu, ctx, torch.empty_like(q), 4, SCALE, ws)
+    seen = torch.ones(300, 300, dtype=torch.bool, device=DEV).tril()
+    exp = attention64(q.view(300, 4, 128), *values[0], seen)
+    top = float(values[0][1].abs().max())
+    err = (out.double() - exp).abs()
+    assert bool((err[1::2] <= exp[1::2].abs() * 2 ** -8 + top * 2 ** -7)[[i for i in range(150) if i != 3]].all())
+    assert bool((err <= exp.abs() * 2 ** -8 + top * 0.5).all()) and bool(out.isfinite().all())
+
+
+def test_prefill_nothing_to_see(ws):
+    """More new tokens than context: rows before the first cached token give zeros."""
+    g = gen(22)
+    cache, tables, values = filled(g, [20], 2, 16, 64)
+    q = torch.randn(200, 2 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    ops.paged_prefill4(q, cache, tables, torch.tensor([0, 200], dtype=torch.int32, device=DEV),
+                       torch.tensor([20], dtype=torch.int32, device=DEV), out, 2, SCALE, ws)
+    assert bool((out[:180] == 0).all())
+    exp = attention64(q[180:].view(20, 2, 128), *values[0], torch.ones(20, 20, dtype=torch.bool, device=DEV).tril())
+    assert bool(((out[180:].double() - exp).abs() <= exp.abs() * 2 ** -8 + float(values[0][1].abs().max()) * 2 ** -7).all())
+
+
+def test_prefill_agrees_with_decode(ws):
+    """The last token of a prefill is a decode over the same cache."""
+    g = gen(23)
+    cache, tables, values = filled(g, [333, 70], 2, 64, 32)
+    ctx = torch.tensor([333, 70], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 8 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    a = ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, ws)
+    b = ops.paged_prefill4(q, cache, tables, torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), ctx,
+                           torch.empty_like(q), 8, SCALE, ws)
+    top = float(values[0][1].abs().max())
+    assert bool(((a.float() - b.float()).abs() <= a.float().abs() * 2 ** -7 + top * 2 ** -7).all())
+
+
+def test_prefill_page_outside_the_cache_is_an_error(ws):
+    g = gen(24)
+    cache, tables, _ = filled(g, [40], 1, 16, 64)
+    tables[0, 1] = -5
+    q = torch.randn(40, 128, generator=g, device=DEV).to(torch.bfloat16)
+    ops.paged_prefill4(q, cache, tables, torch.tensor([0, 40], dtype=torch.int32, device=DEV),
+                       torch.tensor([40], dtype=torch.int32, device=DEV), torch.empty_like(q), 1, SCALE, ws)
     assert ops.check_device_error() != 0
 
 
@@ -325,6 +456,18 @@ def test_refusals(ws):
         a = dict(good, **bad)
         with pytest.raises(ValueError):
             ops.paged_decode4(a["q"], a["cache"], a["tables"], a["ctx"], a["out"], a["heads"], SCALE, a["ws"])
+    with pytest.raises(ValueError):
+        ops.paged_decode4(q, cache, tables, ctx, good["out"], 4, 0.0, ws)
+    cu = torch.arange(3, dtype=torch.int32, device=DEV)
+    good["cu"] = cu
+    ops.paged_prefill4(q, cache, tables, cu, ctx, good["out"], 4, SCALE, ws)
+    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(heads=3), dict(heads=8), dict(tables=tables.long()),
+                dict(tables=tables[:1]), dict(ctx=ctx.long()), dict(ctx=ctx[:1]), dict(ws=ws[:100]), dict(cu=cu.long()),
+                dict(cu=cu[:2]), dict(cu=cu.cpu()), dict(out=q.float()),
+                dict(out=torch.zeros(2, 4 * 128 + 4, dtype=torch.bfloat16, device=DEV)[:, 4:])):
+        a = dict(good, **bad)
+        with pytest.raises(ValueError):
+            ops.paged_prefill4(a["q"], a["cache"], a["tables"], a["cu"], a["ctx"], a["out"], a["heads"], SCALE, a["ws"])
     wide = torch.zeros(2, 34 * 128, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError):
         ops.paged_decode4(wide, cache, tables, ctx, torch.empty_like(wide), 34, SCALE, ws)
