@@ -65,10 +65,30 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
   return d;
 }
 
+__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+
 __device__ __forceinline__ float kv4_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// mbar_wait that polls a while before its limit's clock is read: these kernels'
+// stages turn over in well under a microsecond.
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int code) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity, code);
+}
+
+// Bounded wait that goes on when another wait has given up: for what must end
+// before shared or tensor memory is given back.
+__device__ __forceinline__ void kv4_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kWaitNs) {
+  }
 }
 
 // Online softmax attention of up to 8 * NH query columns (a column = one query
@@ -95,6 +115,7 @@ struct Kv4Warp {
   float acc[NH][8][4];    // sum p s c, channels 16 m + g (+ 8: times 16) x columns 2t, 2t + 1; times 2^-24
   float z[NH][NG][2];     // this lane's share of sum p s z
   float m[NH][2], l[NH][2];
+  float ref[NH][2];       // what scores are taken against: m - KV4_P_BIAS, 0 before the first
 
   // `row(h)` gives the address of column h's 128 query values, null past the last one.
   template <class Row>
@@ -102,56 +123,61 @@ struct Kv4Warp {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
-      float v[4][8];
+      uint32_t x[4][4];                     // 8 channels 32 i + 8 t + 0..7 of column 8 n + g each
       const __nv_bfloat16* src = row(n * 8 + g);
+      __nv_bfloat162 top = __float2bfloat162_rn(0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint4 w = make_uint4(0, 0, 0, 0);
         if (src != nullptr) w = *reinterpret_cast<const uint4*>(src + 32 * i + 8 * t);
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[i][2 * e] = __uint_as_float(x[e] << 16);
-          v[i][2 * e + 1] = __uint_as_float(x[e] & 0xffff0000u);
-        }
+        x[i][0] = w.x;
+        x[i][1] = w.y;
+        x[i][2] = w.z;
+        x[i][3] = w.w;
       }
-      float amax = 0.f, sum[NG];
-#pragma unroll
-      for (int i = 0; i < NG; ++i) sum[i] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          amax = fmaxf(amax, fabsf(v[i][e]));
-          sum[i * NG / 4] += v[i][e];
-        }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-#pragma unroll
-        for (int i = 0; i < NG; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-      }
+        for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x[i][e])));
+      float amax = fmaxf(__low2float(top), __high2float(top));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // amax in [2^e, 2^(e+1)): scale by 2^(14 - e), e kept where that is a normal float
       const int e = min(127, max(-100, (int)((__float_as_uint(amax) >> 23) & 255u) - 127));
       const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
       const float down = up * 0.0625f;
-      const float fh = scale_log2 * exp2f((float)(e + 10));   // 2^24 / up
+      const float fh = scale_log2 * __uint_as_float((uint32_t)min(254, 127 + e + 10) << 23);   // 2^24 / up
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        q[n][2 * i][0] = pack_f16(v[i][0] * up, v[i][4] * up);
-        q[n][2 * i][1] = pack_f16(v[i][1] * down, v[i][5] * down);
-        q[n][2 * i + 1][0] = pack_f16(v[i][2] * up, v[i][6] * up);
-        q[n][2 * i + 1][1] = pack_f16(v[i][3] * down, v[i][7] * down);
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          v[2 * c] = __uint_as_float(x[i][c] << 16);
+          v[2 * c + 1] = __uint_as_float(x[i][c] & 0xffff0000u);
+        }
+        q[n][2 * i][0] = pack_f16(v[0] * up, v[4] * up);
+        q[n][2 * i][1] = pack_f16(v[1] * down, v[5] * down);
+        q[n][2 * i + 1][0] = pack_f16(v[2] * up, v[6] * up);
+        q[n][2 * i + 1][1] = pack_f16(v[3] * down, v[7] * down);
       }
       // the scores' columns are 2t, 2t + 1: fetch those columns' factors
+      f[n][0] = __shfl_sync(0xffffffffu, fh, 8 * t);
+      f[n][1] = __shfl_sync(0xffffffffu, fh, 8 * t + 4);
+      // sums over the groups by the same products, with ones (and 16 for the lowered half) for codes
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8 / NG; ++k)
+          mma_f16(d, 0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u, q[n][i * (8 / NG) + k][0],
+                  q[n][i * (8 / NG) + k][1]);
+        qs[n][i][0] = f[n][0] * 5.9604644775390625e-8f * d[0];   // 2^-24
+        qs[n][i][1] = f[n][1] * 5.9604644775390625e-8f * d[1];
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int from = 4 * (2 * t + c);
-        f[n][c] = __shfl_sync(0xffffffffu, fh, from);
-#pragma unroll
-        for (int i = 0; i < NG; ++i) qs[n][i][c] = scale_log2 * __shfl_sync(0xffffffffu, sum[i], from);
         m[n][c] = -INFINITY;
-        l[n][c] = 0.f;
+        l[n][c] = ref[n][c] = 0.f;
 #pragma unroll
         for (int i = 0; i < NG; ++i) z[n][i][c] = 0.f;
       }
@@ -160,75 +186,85 @@ struct Kv4Warp {
     }
   }
 
-  // One K and V record (`rec` points at K's; 16-byte aligned, shared or global
-  // memory). `seen(token, column)` says whether a column sees token 0..15.
-  template <class Seen>
-  __device__ __forceinline__ void tile(const uint8_t* rec, Seen seen) {
+  // Two K and V records (32 tokens; 16-byte aligned), of which the first `valid`
+  // tokens are seen. An unseen token's weight is 0 whatever its record holds.
+  __device__ __forceinline__ void tokens(const uint8_t* rec, int valid) {
+    if (valid >= 32) tokens_of<true>(rec, 32);
+    else tokens_of<false>(rec, valid);
+  }
+  template <bool ALL>
+  __device__ __forceinline__ void tokens_of(const uint8_t* rec, int valid) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint8_t* vrec = rec + kv4_record(NG);
-    const uint4 k0 = *reinterpret_cast<const uint4*>(rec + g * 64 + t * 16);
-    const uint4 k1 = *reinterpret_cast<const uint4*>(rec + 512 + g * 64 + t * 16);
-    const uint32_t kw0[4] = {k0.x, k0.y, k0.z, k0.w}, kw1[4] = {k1.x, k1.y, k1.z, k1.w};
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(rec + KV4_CODES);
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(vrec + KV4_CODES);
-    float s[NH][4];
+    constexpr int KREC = kv4_record(NG);
+    float s[NH][8];                         // element 4 r + 2 i + c: token 16 r + 8 i + g, column 8 n + 2 t + c
 #pragma unroll
-    for (int n = 0; n < NH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    float zq[NH][4];
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* krec = rec + r * 2 * KREC;
+      const uint4 k0 = *reinterpret_cast<const uint4*>(krec + 16 * lane);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(krec + 512 + 16 * lane);
+      const uint32_t kw0[4] = {k0.x, k0.y, k0.z, k0.w}, kw1[4] = {k1.x, k1.y, k1.z, k1.w};
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(krec + KV4_CODES) + g;
+      float zq[NH][4];
 #pragma unroll
-    for (int n = 0; n < NH; ++n) zq[n][0] = zq[n][1] = zq[n][2] = zq[n][3] = 0.f;
+      for (int ng = 0; ng < NG; ++ng) {
+        float d[NH][4];
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng) {
-      float d[NH][4];
+        for (int n = 0; n < NH; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NH; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+        for (int j = 0; j < 4 / NG; ++j) {
+          const int i = ng * (4 / NG) + j;
+          const uint32_t w0 = kw0[i], w1 = kw1[i], x0 = w0 >> 8, x1 = w1 >> 8;
 #pragma unroll
-      for (int j = 0; j < 4 / NG; ++j) {
-        const int i = ng * (4 / NG) + j;
-        const uint32_t w0 = kw0[i], w1 = kw1[i], x0 = w0 >> 8, x1 = w1 >> 8;
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {
-          mma_f16(d[n], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[n][2 * i][0],
-                  q[n][2 * i][1]);
-          mma_f16(d[n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, q[n][2 * i + 1][0],
-                  q[n][2 * i + 1][1]);
+          for (int n = 0; n < NH; ++n) {
+            mma_f16(d[n], w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, q[n][2 * i][0],
+                    q[n][2 * i][1]);
+            mma_f16(d[n], x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, q[n][2 * i + 1][0],
+                    q[n][2 * i + 1][1]);
+          }
         }
+        const uint32_t p0 = kp[ng * 16], p1 = kp[ng * 16 + 8];
+        const float s0 = kv4_scale(p0), s1 = kv4_scale(p1);
+        const float b0 = s0 * kv4_zero(p0), b1 = s1 * kv4_zero(p1);
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float* v = &s[n][4 * r + c];
+            v[0] = ng == 0 ? s0 * d[n][c] : fmaf(s0, d[n][c], v[0]);
+            v[2] = ng == 0 ? s1 * d[n][2 + c] : fmaf(s1, d[n][2 + c], v[2]);
+            zq[n][c] = ng == 0 ? b0 * qs[n][ng][c] : fmaf(b0, qs[n][ng][c], zq[n][c]);
+            zq[n][2 + c] = ng == 0 ? b1 * qs[n][ng][c] : fmaf(b1, qs[n][ng][c], zq[n][2 + c]);
+          }
       }
-      const uint32_t p0 = kp[ng * 16 + g], p1 = kp[ng * 16 + 8 + g];
-      const float s0 = kv4_scale(p0), s1 = kv4_scale(p1);
-      const float b0 = s0 * kv4_zero(p0), b1 = s1 * kv4_zero(p1);
 #pragma unroll
-      for (int n = 0; n < NH; ++n) {
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          s[n][c] = fmaf(s0, d[n][c], s[n][c]);
-          s[n][2 + c] = fmaf(s1, d[n][2 + c], s[n][2 + c]);
-          zq[n][c] = fmaf(b0, qs[n][ng][c], zq[n][c]);
-          zq[n][2 + c] = fmaf(b1, qs[n][ng][c], zq[n][2 + c]);
+        for (int i = 0; i < 4; ++i) {
+          s[n][4 * r + i] = fmaf(s[n][4 * r + i], f[n][i & 1], zq[n][i]);
+          if (!ALL && 16 * r + 8 * (i >> 1) + g >= valid) s[n][4 * r + i] = -INFINITY;
         }
-      }
     }
+    float top[NH][2];
     bool grow = false;
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int col = n * 8 + 2 * t + c;
-        s[n][c] = seen(g, col) ? fmaf(s[n][c], f[n][c], zq[n][c]) : -INFINITY;
-        s[n][2 + c] = seen(g + 8, col) ? fmaf(s[n][2 + c], f[n][c], zq[n][2 + c]) : -INFINITY;
-        grow |= fmaxf(s[n][c], s[n][2 + c]) > m[n][c] + KV4_LAZY;
+        top[n][c] = fmaxf(fmaxf(s[n][c], s[n][2 + c]), fmaxf(s[n][4 + c], s[n][6 + c]));
+        grow |= top[n][c] > m[n][c] + KV4_LAZY;
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(s[n][c], s[n][2 + c]);
+          float mx = top[n][c];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
           mx = fmaxf(mx, m[n][c]);
           const float corr = mx == -INFINITY ? 1.f : kv4_exp2(m[n][c] - mx);
           m[n][c] = mx;
+          ref[n][c] = mx == -INFINITY ? 0.f : mx - KV4_P_BIAS;
           l[n][c] *= corr;
 #pragma unroll
           for (int i = 0; i < NG; ++i) z[n][i][c] *= corr;
@@ -242,49 +278,52 @@ struct Kv4Warp {
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float ref = m[n][c] == -INFINITY ? 0.f : m[n][c] - KV4_P_BIAS;
-        s[n][c] = kv4_exp2(s[n][c] - ref);
-        s[n][2 + c] = kv4_exp2(s[n][2 + c] - ref);
-        l[n][c] += s[n][c] + s[n][2 + c];
-      }
+      for (int i = 0; i < 8; ++i) s[n][i] = kv4_exp2(s[n][i] - ref[n][i & 1]);
 #pragma unroll
-    for (int ng = 0; ng < NG; ++ng) {
-      const uint32_t p0 = vp[ng * 16 + g], p1 = vp[ng * 16 + 8 + g];
-      const float s0 = kv4_scale(p0), s1 = kv4_scale(p1);
-      const float b0 = s0 * kv4_zero(p0), b1 = s1 * kv4_zero(p1);
-      uint32_t w[NH][2];
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        // an unseen token's weight is 0 whatever its record holds
-        float u[4];
+      for (int c = 0; c < 2; ++c) l[n][c] += (s[n][c] + s[n][2 + c]) + (s[n][4 + c] + s[n][6 + c]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const bool on0 = s[n][c] != 0.f, on1 = s[n][2 + c] != 0.f;
-          u[c] = on0 ? s[n][c] * s0 : 0.f;
-          u[2 + c] = on1 ? s[n][2 + c] * s1 : 0.f;
-          z[n][ng][c] += (on0 ? s[n][c] * b0 : 0.f) + (on1 ? s[n][2 + c] * b1 : 0.f);
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* vrec = rec + r * 2 * KREC + KREC;
+      const uint4 v0 = *reinterpret_cast<const uint4*>(vrec + 16 * lane);
+      const uint4 v1 = *reinterpret_cast<const uint4*>(vrec + 512 + 16 * lane);
+      const uint32_t vw[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(vrec + KV4_CODES) + g;
+#pragma unroll
+      for (int ng = 0; ng < NG; ++ng) {
+        uint32_t p0 = vp[ng * 16], p1 = vp[ng * 16 + 8];
+        if (!ALL && 16 * r + g >= valid) p0 = 0;
+        if (!ALL && 16 * r + g + 8 >= valid) p1 = 0;
+        const float s0 = kv4_scale(p0), s1 = kv4_scale(p1);
+        const float b0 = s0 * kv4_zero(p0), b1 = s1 * kv4_zero(p1);
+        uint32_t w[NH][2];
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          const float* p = &s[n][4 * r];
+          w[n][0] = movm_t(pack_f16(p[0] * s0, p[1] * s0));
+          w[n][1] = movm_t(pack_f16(p[2] * s1, p[3] * s1));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) z[n][ng][c] = fmaf(p[c], b0, fmaf(p[2 + c], b1, z[n][ng][c]));
         }
-        w[n][0] = movm_t(pack_f16(u[0], u[1]));
-        w[n][1] = movm_t(pack_f16(u[2], u[3]));
-      }
 #pragma unroll
-      for (int j = 0; j < 8 / NG; ++j) {
-        const int i = ng * (8 / NG) + j;
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(vrec + 512 * (i / 4) + 16 * lane + 4 * (i % 4));
-        const uint32_t y = x >> 8;
+        for (int j = 0; j < 8 / NG; ++j) {
+          const int i = ng * (8 / NG) + j;
+          const uint32_t x = vw[i], y = x >> 8;
 #pragma unroll
-        for (int n = 0; n < NH; ++n)
-          mma_f16(acc[n][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, w[n][0], w[n][1]);
+          for (int n = 0; n < NH; ++n)
+            mma_f16(acc[n][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, w[n][0], w[n][1]);
+        }
       }
     }
   }
 
-  // Sum the lanes' shares; afterwards `out(n, i, e)` is the unnormalised output
-  // of channel 16 i + g + 8 (e / 2), column 8 n + 2 t + e % 2.
+  // Sum the lanes' shares and complete the output: afterwards acc[n][i][e] is
+  // the unnormalised output of channel 16 i + g + 8 (e / 2), column
+  // 8 n + 2 t + e % 2.
   __device__ __forceinline__ void finish() {
 #pragma unroll
-    for (int n = 0; n < NH; ++n)
+    for (int n = 0; n < NH; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -293,9 +332,92 @@ struct Kv4Warp {
 #pragma unroll
           for (int i = 0; i < NG; ++i) z[n][i][c] += __shfl_xor_sync(0xffffffffu, z[n][i][c], o);
         }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[n][i][e] = fmaf(acc[n][i][e], e < 2 ? 16777216.f : 1048576.f, z[n][i * NG / 8][e & 1]);
+    }
   }
-  __device__ __forceinline__ float out(int n, int i, int e) const {
-    return fmaf(acc[n][i][e], e < 2 ? 16777216.f : 1048576.f, z[n][i * NG / 8][e & 1]);
+
+  // A finished state as 9 NH rows of one float4 per lane: (m, m, l, l), then the
+  // eight tiles, for each n.
+  static constexpr int PART = 9 * NH * 32;   // float4s
+  __device__ __forceinline__ void save(float4* part) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      __stcg(part + 9 * n * 32 + lane, make_float4(m[n][0], m[n][1], l[n][0], l[n][1]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        __stcg(part + (9 * n + 1 + i) * 32 + lane, make_float4(acc[n][i][0], acc[n][i][1], acc[n][i][2], acc[n][i][3]));
+    }
+  }
+  // Join up to eight saved states, in order. part(x): the x-th one.
+  template <class Part>
+  __device__ __forceinline__ void join(int count, Part part) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll 4
+      for (int x = 0; x < count; ++x) {
+        const float4 ml = __ldcg(part(x) + 9 * n * 32 + lane);
+        m0 = fmaxf(m0, ml.x);
+        m1 = fmaxf(m1, ml.y);
+      }
+      m[n][0] = m0;
+      m[n][1] = m1;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+#pragma unroll 2
+      for (int x = 0; x < count; ++x) {
+        const float4* p = part(x) + 9 * n * 32 + lane;
+        const float4 ml = __ldcg(p);
+        float4 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = __ldcg(p + 32 * (i + 1));
+        // a part that saw no token counts nothing (a NaN sum goes on)
+        const float e0 = ml.z == 0.f ? 0.f : kv4_exp2(ml.x - m0), e1 = ml.w == 0.f ? 0.f : kv4_exp2(ml.y - m1);
+        l[n][0] += ml.z * e0;
+        l[n][1] += ml.w * e1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          acc[n][i][0] = fmaf(o[i].x, e0, acc[n][i][0]);
+          acc[n][i][1] = fmaf(o[i].y, e1, acc[n][i][1]);
+          acc[n][i][2] = fmaf(o[i].z, e0, acc[n][i][2]);
+          acc[n][i][3] = fmaf(o[i].w, e1, acc[n][i][3]);
+        }
+      }
+    }
+  }
+
+  // Normalise and store as bf16: column c's row is out + c * HD, `cols` columns
+  // (VEC: rows are 4-byte aligned). A column that saw no token gives zeros.
+  template <bool VEC>
+  __device__ __forceinline__ void store(__nv_bfloat16* out, int cols) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const float i0 = l[n][0] != 0.f ? 1.f / l[n][0] : 0.f, i1 = l[n][1] != 0.f ? 1.f / l[n][1] : 0.f;
+      // the transposed tile has column g's channels 2t, 2t + 1 side by side
+      __nv_bfloat16* dst = out + (n * 8 + g) * HD + 2 * t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = movm_t(pack_bf16(acc[n][i][2 * h] * i0, acc[n][i][2 * h + 1] * i1));
+          if (n * 8 + g < cols) {
+            if (VEC) {
+              *reinterpret_cast<uint32_t*>(dst + 16 * i + 8 * h) = w;
+            } else {
+              reinterpret_cast<uint16_t*>(dst + 16 * i + 8 * h)[0] = (uint16_t)w;
+              reinterpret_cast<uint16_t*>(dst + 16 * i + 8 * h)[1] = (uint16_t)(w >> 16);
+            }
+          }
+        }
+    }
   }
 };
 

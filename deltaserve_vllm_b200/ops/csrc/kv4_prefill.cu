@@ -62,7 +62,6 @@ enum : int {
   kErrP4O = 0x4405,
   kErrP4KEmpty = 0x4406,
   kErrP4VEmpty = 0x4407,
-  kErrP4Drain = 0x4408,
 };
 
 struct Prefill4Args {
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
     bool ok = true;
     const int n = n_kb[x];
     for (int j = 0; j < n; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], (uint32_t)j & 1u, kErrP4S))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, kv4_wait(&s_full[x], (uint32_t)j & 1u, kErrP4S))) { ok = false; break; }
       tc_fence_after();
       float s[128];
       {
@@ -312,7 +311,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       tc_fence_before();
       mbar_arrive(&p_full[x]);
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], 0, kErrP4O));
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, kv4_wait(&o_done[x], 0, kErrP4O));
     if (ok) {
       tc_fence_after();
       const float inv = l != 0.f ? 1.f / l : 0.f;           // a row that sees no key gives zeros
@@ -385,7 +384,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
     for (int j = 0; j < n_max; ++j) {
       const int st = j & 1;
       const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u;
-      if (!__all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph, kErrP4KEmpty))) break;
+      if (!__all_sync(0xffffffffu, kv4_wait(&k_empty[st], ph, kErrP4KEmpty))) break;
       {
         uint8_t* dst = sK + st * P4_TILE + key * 128;
 #pragma unroll
@@ -406,7 +405,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       if (j + 1 < n_max) load_k(j + 1);
       fence_proxy_async_smem();
       mbar_arrive(&k_full[st]);
-      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph, kErrP4VEmpty))) break;
+      if (!__all_sync(0xffffffffu, kv4_wait(&v_empty[st], ph, kErrP4VEmpty))) break;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int rec = w4 * 2 + b;
@@ -457,8 +456,8 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         tc_commit(&s_full[x]);
       };
       auto output = [&](int x, int j) -> bool {
-        if (!mbar_wait(&p_full[x], (uint32_t)j & 1u, kErrP4P)) return false;
-        if (!mbar_wait(&v_full[j & 1], (uint32_t)(j >> 1) & 1u, kErrP4V)) return false;
+        if (!kv4_wait(&p_full[x], (uint32_t)j & 1u, kErrP4P)) return false;
+        if (!kv4_wait(&v_full[j & 1], (uint32_t)(j >> 1) & 1u, kErrP4V)) return false;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
@@ -467,7 +466,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         if (j == n_kb[x] - 1) tc_commit(&o_done[x]);
         return true;
       };
-      bool ok = mbar_wait(&k_full[0], 0, kErrP4K);
+      bool ok = kv4_wait(&k_full[0], 0, kErrP4K);
       if (ok) {
         tc_fence_after();
         if (n_kb[0] > 0) scores(0, 0);
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         if (j < n_kb[0] && !output(0, j)) break;
         const bool more = j + 1 < n_max;
         if (more) {
-          if (!mbar_wait(&k_full[(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1u, kErrP4K)) break;
+          if (!kv4_wait(&k_full[(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1u, kErrP4K)) break;
           tc_fence_after();
           if (j + 1 < n_kb[0]) scores(0, j + 1);
         }
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       }
       // Every product has finished before the CTA gives its memory back.
       tc_commit(drain);
-      mbar_wait(drain, 0, kErrP4Drain);
+      kv4_drain(drain, 0);
     }
   }
   tc_fence_before();
