@@ -52,6 +52,7 @@ constexpr int P4_CHUNK = 128 * 128;          // [128 rows x 64 columns] fp16, by
 constexpr int P4_TILE = 2 * P4_CHUNK;
 constexpr int P4_SMEM = 6 * P4_TILE + 1024 + 256 * 4 + 256;
 constexpr float P4_LAZY = 8.f;
+constexpr int P4_PART = HD + 4;              // floats of a row's partial result
 constexpr uint32_t P4_IDESC = (1u << 4) | (128u >> 3) << 17 | (128u >> 4) << 24;   // f16 x f16 -> f32, 128 x 128
 
 enum : int {
@@ -75,6 +76,8 @@ struct Prefill4Args {
   int64_t out_stride;
   int seqs, rows, max_pages, num_pages, kv_heads, group, sub;
   int tile_rows;            // query rows per CTA: 128 or 256
+  int splits;               // CTAs that share a tile's keys (128-row tiles only)
+  float* part;              // [grid x, Hkv, splits, 128 rows, P4_PART]: unnormalised output, maximum, sum
   float scale_log2;
 };
 
@@ -91,6 +94,24 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, 
       : "memory");
 }
 
+// 32 lanes x 16 columns (common.cuh has the 32-column forms): the softmax warps
+// have no 32 registers to spare beside a row of scores.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void reg_grow() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -100,13 +121,69 @@ __device__ __forceinline__ void reg_shrink() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// s (c + z) of the code pair at bits 0-3 of w's halves, after `w` was shifted
-// so that the pair lies at bits 6-9: 64 + 4 c by mask, 4 c exactly, one rounding.
-__device__ __forceinline__ uint32_t p4_value(uint32_t w, __half2 quarter, __half2 base) {
-  const uint32_t m = (w & 0x03c003c0u) | 0x54005400u;
-  const __half2 c4 = __hsub2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(64.f));
-  const __half2 v = __hfma2(c4, quarter, base);
-  return *reinterpret_cast<const uint32_t*>(&v);
+struct P4Tile {
+  int seq, local;           // sequence (-1: past the last tile) and which of its query tiles
+};
+// The `left`-th tile of the packed sequences: a sequence's last, longest tile first.
+__device__ __forceinline__ P4Tile p4_tile(const Prefill4Args& a, int left) {
+  const int lane = threadIdx.x & 31;
+  for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+    int n = 0;
+    if (s0 + lane < a.seqs) {
+      const int len = a.cu_q[s0 + lane + 1] - a.cu_q[s0 + lane];
+      n = len > 0 ? (len * a.group + a.tile_rows - 1) / a.tile_rows : 0;
+    }
+    int up = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, up > left);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      return {s0 + at, __shfl_sync(0xffffffffu, up, at) - 1 - left};
+    }
+    left -= __shfl_sync(0xffffffffu, up, 31);
+  }
+  return {-1, 0};
+}
+
+// The values s (c + z) of a word's eight codes as four pairs (code i, code i + 4):
+// 1024 + c (1024 + 16 c) by mask, c exactly, then one rounding.
+__device__ __forceinline__ void p4_values(uint32_t w, __half2 s, __half2 sz, uint32_t (&v)[4]) {
+  const __half2 big = __float2half2_rn(1024.f), low = __float2half2_rn(-64.f), part = __float2half2_rn(0.0625f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t m0 = (w & 0x000f000fu) | 0x64006400u, m1 = (w & 0x00f000f0u) | 0x64006400u;
+    const __half2 c0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), big);
+    const __half2 c1 = __hfma2(*reinterpret_cast<const __half2*>(&m1), part, low);
+    const __half2 v0 = __hfma2(c0, s, sz), v1 = __hfma2(c1, s, sz);
+    v[2 * i] = *reinterpret_cast<const uint32_t*>(&v0);
+    v[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&v1);
+    w >>= 8;
+  }
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 template <int NG>
@@ -131,30 +208,8 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kvh = blockIdx.y;
 
-  // Which sequence, and which of its query tiles (the last, longest first).
-  int seq = -1, local = 0, left = blockIdx.x;
-  for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-    int n = 0;
-    if (s0 + lane < a.seqs) {
-      const int len = a.cu_q[s0 + lane + 1] - a.cu_q[s0 + lane];
-      n = len > 0 ? (len * a.group + a.tile_rows - 1) / a.tile_rows : 0;
-    }
-    int up = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += x;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, up > left);
-    if (past != 0) {
-      const int at = __ffs(past) - 1;
-      const int end = __shfl_sync(0xffffffffu, up, at);
-      seq = s0 + at;
-      local = end - 1 - left;
-      break;
-    }
-    left -= __shfl_sync(0xffffffffu, up, 31);
-  }
+  const P4Tile tile = p4_tile(a, blockIdx.x);
+  const int seq = tile.seq, local = tile.local;
   if (seq < 0) return;
   const int q_begin = a.cu_q[seq], q_len = a.cu_q[seq + 1] - q_begin;
   const int ctx = min(a.ctx[seq], a.max_pages * a.sub * 16);
@@ -168,6 +223,13 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
   for (int x = 0; x < 2; ++x) {
     const int last = min(rows, (x + 1) * 128) - 1;
     n_kb[x] = last >= x * 128 ? max(0, pos0 + (row0 + last) / a.group + 1 + 127) / 128 : 0;
+  }
+  // this split's key tiles: kb0 onwards
+  int kb0 = 0;
+  if (a.splits > 1) {
+    const int per = max(2, (n_kb[0] + a.splits - 1) / a.splits);
+    kb0 = (int)blockIdx.z * per;
+    n_kb[0] = max(0, min(per, n_kb[0] - kb0));
   }
   const int n_max = max(n_kb[0], n_kb[1]);
   const int kv_end = pos0 + (row0 + rows - 1) / a.group + 1;
@@ -260,19 +322,18 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
           s[96 + i] = __uint_as_float(v3[i]);
         }
       }
-      const int lim = seen - j * 128;
+      const int lim = seen - (kb0 + j) * 128;
       if (__any_sync(0xffffffffu, lim < 128)) {
 #pragma unroll
         for (int i = 0; i < 128; ++i)
           if (i >= lim) s[i] = -INFINITY;
       }
-      float red[8];
+      float red[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) red[c] = s[c];
+      for (int c = 0; c < 4; ++c) red[c] = fmaxf(s[2 * c], s[2 * c + 1]);
 #pragma unroll
-      for (int i = 8; i < 128; ++i) red[i & 7] = fmaxf(red[i & 7], s[i]);
-      const float row_max = f * fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])),
-                                      fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])));
+      for (int i = 8; i < 128; i += 2) red[i / 2 & 3] = max3(red[i / 2 & 3], s[i], s[i + 1]);
+      const float row_max = f * fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
       // The reference maximum moves only when it is exceeded by 2^8: P stays
       // below 2^8 in fp16 and the common factor cancels in O / l.
       const bool move = m == -INFINITY || row_max > m + P4_LAZY;
@@ -284,35 +345,53 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       // s_full of this tile was committed after the last product into O
       if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t_o + c * 32, v);
+        for (int c = 0; c < 8; ++c) {
+          uint32_t v[16];
+          tmem_ld_x16(t_o + c * 16, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-          tmem_st_32x32b_x32(t_o + c * 32, v);
+          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+          tmem_st_x16(t_o + c * 16, v);
         }
       }
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 f2 = make_float2(f, f), r2 = make_float2(-ref, -ref);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p0 = kv4_exp2(fmaf(s[c * 64 + 2 * i], f, -ref)), p1 = kv4_exp2(fmaf(s[c * 64 + 2 * i + 1], f, -ref));
-          sum[(2 * i) & 3] += p0;
-          sum[(2 * i + 1) & 3] += p1;
-          p[i] = pack_f16(p0, p1);
+        for (int i = 0; i < 16; ++i) {
+          float2 e = fma2(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), f2, r2);
+          e = make_float2(kv4_exp2(e.x), kv4_exp2(e.y));
+          sum[i & 1] = add2(sum[i & 1], e);
+          p[i] = pack_f16(e.x, e.y);
         }
-        tmem_st_32x32b_x32(t_s + c * 32, p);
+        tmem_st_x16(t_s + c * 16, p);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sum[0] = add2(sum[0], sum[1]);
+      l += sum[0].x + sum[0].y;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_full[x]);
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, kv4_wait(&o_done[x], 0, kErrP4O));
-    if (ok) {
+    if (ok && a.splits > 1) {
+      tc_fence_after();
+      float* dst = a.part + ((((size_t)blockIdx.x * a.kv_heads + kvh) * a.splits + blockIdx.z) * 128 + r) * P4_PART;
+      if (x == 0) {
+        *reinterpret_cast<float2*>(dst + HD) = make_float2(m, l);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (n == 0) break;
+          uint32_t v[16];
+          tmem_ld_x16(t_o + c * 16, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(dst + c * 16 + u * 4) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        }
+      }
+    } else if (ok) {
       tc_fence_after();
       const float inv = l != 0.f ? 1.f / l : 0.f;           // a row that sees no key gives zeros
       __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
@@ -343,43 +422,66 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
     // -------------------------------------------------------------- dequantise
     reg_shrink<88>();
     const int w4 = warp - 8;
-    const int key = w4 * 32 + lane;                        // K: this thread's key of the tile
+    // The warp's 32 keys of a tile are two records; lane l has token l % 16 of
+    // record l / 16: its K row, and its K and V scales and zero points.
+    const int key = w4 * 32 + lane;
     const int g = lane >> 2, t = lane & 3;
-    auto record = [&](int rec) -> const uint8_t* {          // K record of 16-token block `rec`; null past the end
-      if (rec * 16 >= kv_end) return nullptr;
-      const int page = tab[rec / a.sub];
-      if ((unsigned)page >= (unsigned)a.num_pages) {
-        set_error(kErrShape);
-        return nullptr;
-      }
-      return a.cache + (((size_t)page * a.kv_heads + kvh) * a.sub + rec % a.sub) * (2 * kv4_record(NG));
-    };
     uint4 kc[4], vc[2][2];
-    uint32_t kp[NG];
-    const uint8_t* vrec[2];
-    auto load_k = [&](int j) {
-      const uint8_t* p = record(j * 8 + key / 16);
-      if (p != nullptr && j * 128 + key >= kv_end) p = nullptr;
+    uint32_t kp[NG], vp[NG];
+    // The record's place, moved by a tile (8 records) at a time, and its page a tile ahead of its use.
+    const int step_page = 8 / a.sub, step_off = 8 % a.sub;
+    int at_key = kb0 * 128 + key;
+    int at_page = (at_key / 16) / a.sub, at_off = (at_key / 16) % a.sub;
+    int page = 0;
+    const uint8_t* rec = nullptr;               // of the tile to load; null past the end
+    bool in = false;                            // its token exists
+    auto next = [&]() {                         // the looked-up record's address, then the next look-up
+      rec = nullptr;
+      in = at_key < kv_end;
+      if (at_key - (lane & 15) < kv_end) {
+        if ((unsigned)page >= (unsigned)a.num_pages) {              // read another page instead, and say so
+          set_error(kErrShape);
+          page = 0;
+        }
+        rec = a.cache + (((size_t)page * a.kv_heads + kvh) * a.sub + at_off) * (2 * kv4_record(NG));
+      }
+      at_key += 128;
+      at_page += step_page;
+      at_off += step_off;
+      if (at_off >= a.sub) {
+        at_off -= a.sub;
+        ++at_page;
+      }
+      if (at_key - (lane & 15) < kv_end) page = tab[at_page];
+    };
+    auto load_k = [&]() {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        kc[i] = p != nullptr ? *reinterpret_cast<const uint4*>(p + (key & 15) * 64 + i * 16) : make_uint4(0, 0, 0, 0);
+        kc[i] = in ? *reinterpret_cast<const uint4*>(rec + (lane & 15) * 64 + i * 16) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < NG; ++i)
-        kp[i] = p != nullptr ? *reinterpret_cast<const uint32_t*>(p + KV4_CODES + 64 * i + 4 * (key & 15)) : 0u;
+        kp[i] = in ? *reinterpret_cast<const uint32_t*>(rec + KV4_CODES + 64 * i + 4 * (lane & 15)) : 0u;
     };
-    auto load_v = [&](int j) {
+    auto load_v = [&]() {
+      const uint8_t* v = rec != nullptr ? rec + kv4_record(NG) : nullptr;
+      // a key that no query sees is a zero row whatever its record holds
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+        vp[i] = in ? *reinterpret_cast<const uint32_t*>(v + KV4_CODES + 64 * i + 4 * (lane & 15)) : 0u;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        vrec[b] = record(j * 8 + w4 * 2 + b);
-        if (vrec[b] != nullptr) vrec[b] += kv4_record(NG);
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(v), 16 * b));
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          vc[b][i] = vrec[b] != nullptr ? *reinterpret_cast<const uint4*>(vrec[b] + i * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
+          vc[b][i] = p != nullptr ? *reinterpret_cast<const uint4*>(p + i * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
       }
     };
     if (n_max > 0) {
-      load_k(0);
-      load_v(0);
+      if (at_key - (lane & 15) < kv_end) page = tab[at_page];
+      next();
+      load_k();
+      load_v();
     }
     for (int j = 0; j < n_max; ++j) {
       const int st = j & 1;
@@ -388,60 +490,68 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       {
         uint8_t* dst = sK + st * P4_TILE + key * 128;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                       // 16-byte words of lane t = i: word e covers channels 32 e + 8 i
-          const uint32_t x[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
+        for (int i = 0; i < NG; ++i) {
+          const __half2 sc = __float2half2_rn(kv4_scale(kp[i]));
+          const __half2 sz = __float2half2_rn(kv4_scale(kp[i]) * kv4_zero(kp[i]));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t pw = kp[e * NG / 4];
-            const __half2 quarter = __float2half2_rn(kv4_scale(pw) * 0.25f);
-            const __half2 base = __float2half2_rn(kv4_scale(pw) * kv4_zero(pw));
-            const int u = 4 * e + i;                        // 16-byte unit of the row
-            *reinterpret_cast<uint4*>(dst + (u >> 3) * P4_CHUNK + (((u & 7) ^ (key & 7)) << 4)) =
-                make_uint4(p4_value(x[e] << 6, quarter, base), p4_value(x[e] << 2, quarter, base),
-                           p4_value(x[e] >> 2, quarter, base), p4_value(x[e] >> 6, quarter, base));
-          }
+          for (int e = i * (4 / NG); e < (i + 1) * (4 / NG); ++e)   // word e of 16 bytes h: channels 32 e + 8 h
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const uint32_t w = e == 0 ? kc[h].x : e == 1 ? kc[h].y : e == 2 ? kc[h].z : kc[h].w;
+              uint32_t v[4];
+              p4_values(w, sc, sz, v);
+              const int u = 4 * e + h;                      // 16-byte unit of the row
+              *reinterpret_cast<uint4*>(dst + (u >> 3) * P4_CHUNK + (((u & 7) ^ (key & 7)) << 4)) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
+            }
         }
       }
-      if (j + 1 < n_max) load_k(j + 1);
       fence_proxy_async_smem();
       mbar_arrive(&k_full[st]);
+      if (j + 1 < n_max) {
+        next();
+        load_k();
+      }
+      uint32_t ss[NG];                                      // fp16 (scale, scale x zero point) of this lane's token
+#pragma unroll
+      for (int i = 0; i < NG; ++i) ss[i] = pack_f16(kv4_scale(vp[i]), kv4_scale(vp[i]) * kv4_zero(vp[i]));
       if (!__all_sync(0xffffffffu, kv4_wait(&v_empty[st], ph, kErrP4VEmpty))) break;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int rec = w4 * 2 + b;
-        const int tok = j * 128 + rec * 16 + 2 * t;         // tokens tok, tok + 1, tok + 8, tok + 9
-        uint8_t* dst = sV + st * P4_TILE + (rec >> 2) * P4_CHUNK + g * 128 + 4 * t;
-        const int u = 2 * (rec & 3);                        // 16-byte unit (8 tokens) of the row; u + 1 the late half
-        const uint32_t x[8] = {vc[b][0].x, vc[b][0].y, vc[b][0].z, vc[b][0].w,
-                               vc[b][1].x, vc[b][1].y, vc[b][1].z, vc[b][1].w};
+        const int r = w4 * 2 + b;                           // record of the tile
+        uint8_t* dst = sV + st * P4_TILE + (r >> 2) * P4_CHUNK + g * 128 + 4 * t;
+        const int u = 2 * (r & 3);                          // 16-byte unit (8 tokens) of the row; u + 1 the late half
+        uint8_t* d0 = dst + ((u ^ g) << 4);
+        uint8_t* d1 = dst + (((u + 1) ^ g) << 4);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          __half2 quarter[2], base[2];
+          // (scale, scale) and (base, base) of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+          uint32_t sc[2], sz[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint2 pw = make_uint2(0, 0);
-            if (vrec[b] != nullptr) pw = *reinterpret_cast<const uint2*>(vrec[b] + KV4_CODES + 64 * i + 8 * t + 32 * h);
-            // a key that no query sees is a zero row whatever its record holds
-            if (tok + 8 * h >= kv_end) pw.x = 0;
-            if (tok + 8 * h + 1 >= kv_end) pw.y = 0;
-            const float s0 = kv4_scale(pw.x), s1 = kv4_scale(pw.y);
-            quarter[h] = __floats2half2_rn(s0 * 0.25f, s1 * 0.25f);
-            base[h] = __floats2half2_rn(s0 * kv4_zero(pw.x), s1 * kv4_zero(pw.y));
+            const uint32_t x = __shfl_sync(0xffffffffu, ss[i], 16 * b + 8 * h + 2 * t);
+            const uint32_t y = __shfl_sync(0xffffffffu, ss[i], 16 * b + 8 * h + 2 * t + 1);
+            sc[h] = __byte_perm(x, y, 0x5410);
+            sz[h] = __byte_perm(x, y, 0x7632);
           }
 #pragma unroll
           for (int q = 0; q < 8 / NG; ++q) {
             const int mt = i * (8 / NG) + q;                // channels 16 mt + g and + 8
-            uint8_t* d0 = dst + mt * 2048;
-            *reinterpret_cast<uint32_t*>(d0 + ((u ^ g) << 4)) = p4_value(x[mt] << 6, quarter[0], base[0]);
-            *reinterpret_cast<uint32_t*>(d0 + 1024 + ((u ^ g) << 4)) = p4_value(x[mt] << 2, quarter[0], base[0]);
-            *reinterpret_cast<uint32_t*>(d0 + (((u + 1) ^ g) << 4)) = p4_value(x[mt] >> 2, quarter[1], base[1]);
-            *reinterpret_cast<uint32_t*>(d0 + 1024 + (((u + 1) ^ g) << 4)) = p4_value(x[mt] >> 6, quarter[1], base[1]);
+            const uint4& c = vc[b][mt / 4];
+            const uint32_t w = mt % 4 == 0 ? c.x : mt % 4 == 1 ? c.y : mt % 4 == 2 ? c.z : c.w;
+            uint32_t v[4], late[4];
+            p4_values(w, *reinterpret_cast<const __half2*>(&sc[0]), *reinterpret_cast<const __half2*>(&sz[0]), v);
+            p4_values(w, *reinterpret_cast<const __half2*>(&sc[1]), *reinterpret_cast<const __half2*>(&sz[1]), late);
+            *reinterpret_cast<uint32_t*>(d0 + mt * 2048) = v[0];
+            *reinterpret_cast<uint32_t*>(d0 + mt * 2048 + 1024) = v[1];
+            *reinterpret_cast<uint32_t*>(d1 + mt * 2048) = late[2];
+            *reinterpret_cast<uint32_t*>(d1 + mt * 2048 + 1024) = late[3];
           }
         }
       }
-      if (j + 1 < n_max) load_v(j + 1);
       fence_proxy_async_smem();
       mbar_arrive(&v_full[st]);
+      if (j + 1 < n_max) load_v();
     }
   } else {
     reg_shrink<40>();
@@ -501,6 +611,39 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
   }
 }
 
+// Joins the splits of a tile: one warp per row, four channels per lane.
+// grid (tile, KV head, 16), 8 rows per CTA.
+__global__ void __launch_bounds__(256) prefill4_join_kernel(const Prefill4Args a) {
+  const P4Tile tile = p4_tile(a, blockIdx.x);
+  if (tile.seq < 0) return;
+  const int lane = threadIdx.x & 31, kvh = blockIdx.y;
+  const int r = blockIdx.z * 8 + threadIdx.x / 32;
+  const int q_begin = a.cu_q[tile.seq], q_len = a.cu_q[tile.seq + 1] - q_begin;
+  const int row = tile.local * 128 + r;
+  if (row >= q_len * a.group) return;
+  const float* part = a.part + ((((size_t)blockIdx.x * a.kv_heads + kvh) * a.splits) * 128 + r) * P4_PART;
+  const size_t step = (size_t)128 * P4_PART;
+  float M = -INFINITY, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, part[s * step + HD]);
+#pragma unroll 8
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(part + s * step + HD);
+    const float4 v = *reinterpret_cast<const float4*>(part + s * step + 4 * lane);
+    if (ml.y == 0.f) continue;               // saw no key (a NaN sum goes on)
+    const float e = kv4_exp2(ml.x - M);
+    L += ml.y * e;
+    o.x = fmaf(v.x, e, o.x);
+    o.y = fmaf(v.y, e, o.y);
+    o.z = fmaf(v.z, e, o.z);
+    o.w = fmaf(v.w, e, o.w);
+  }
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
+                       (int64_t)(kvh * a.group + row % a.group) * HD + 4 * lane;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+}
+
 template <int NG>
 static void prefill4_launch(const Prefill4Args& a, dim3 grid, cudaStream_t stream) {
   static const cudaError_t attr =
@@ -508,6 +651,10 @@ static void prefill4_launch(const Prefill4Args& a, dim3 grid, cudaStream_t strea
   C10_CUDA_CHECK(attr);
   prefill4_kernel<NG><<<grid, P4_THREADS, P4_SMEM, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    prefill4_join_kernel<<<dim3(grid.x, grid.y, 16), 256, 0, stream>>>(a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
 }
 
 }  // namespace dsv
@@ -562,13 +709,21 @@ int64_t dsv_paged_prefill4(torch::Tensor q, torch::Tensor cache, torch::Tensor t
   // Two tiles per CTA share the dequantised keys; with too few of them to fill
   // the SMs, one tile per CTA.
   const int64_t all = q.size(0) * a.group;
-  a.tile_rows = all / 256 * hkv >= at::cuda::getCurrentDeviceProperties()->multiProcessorCount ? 256 : 128;
-  const dim3 grid((unsigned)(all / a.tile_rows + a.seqs), (unsigned)hkv);
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  a.tile_rows = all / 256 * hkv >= sms ? 256 : 128;
+  // With tiles for less than half of the SMs, several CTAs share a tile's keys
+  // (where the tables allow a context of several key tiles at all).
+  const int64_t tiles = all / a.tile_rows + a.seqs, most = (int64_t)a.max_pages * a.sub / 16;
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(sms / (tiles * hkv), std::min<int64_t>(most, 32)));
+  a.part = reinterpret_cast<float*>(ws.data_ptr());
+  TORCH_CHECK(a.splits == 1 || tiles * hkv * a.splits * 128 * P4_PART * 4 <= dsv_kv4_workspace_bytes() - (1 << 20),
+              "paged_prefill4: workspace too small for this GPU");
+  const dim3 grid((unsigned)tiles, (unsigned)hkv, (unsigned)a.splits);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (ng == 1) prefill4_launch<1>(a, grid, stream);
   else if (ng == 2) prefill4_launch<2>(a, grid, stream);
   else prefill4_launch<4>(a, grid, stream);
-  return 1;
+  return a.splits > 1 ? 2 : 1;
 }
 
 DSV_ERROR_ACCESSOR(dsv_read_error_kv4_prefill)

@@ -353,6 +353,12 @@ def test_prefill_both_tile_widths(ws):
     check_prefill(new, old, 16, 8, 64, 64, ws, q=q)
 
 
+@pytest.mark.parametrize("new,old", [([5], [3000]), ([33, 1], [1500, 130]), ([64], [1]), ([128], [2000])])
+def test_prefill_few_rows_split_their_keys(new, old, ws):
+    """Too few tiles for the SMs: several CTAs share a long context, some of them past its end."""
+    check_prefill(new, old, 4, 1, 64, 64, ws)
+
+
 def test_prefill_many_short_sequences(ws):
     check_prefill([1 + i % 5 for i in range(90)], [i % 41 for i in range(90)], 4, 2, 16, 64, ws)
 
