@@ -275,6 +275,10 @@ class EngineConfig:
     # KV cache: page size in tokens and the share of free HBM it may take.
     block_size: int = 64
     gpu_memory_utilization: float = 0.85
+    # What the cache holds: "auto" = the compute dtype, "int4" = 4-bit codes with
+    # a scale and a zero point per ``kv_cache_group`` channels (head_dim 128).
+    kv_cache_dtype: str = "auto"
+    kv_cache_group: int = 64
     num_gpu_blocks_override: int | None = None
     max_num_seqs: int = 256
     max_num_batched_tokens: int = 8192
@@ -306,6 +310,9 @@ class EngineConfig:
         if self.block_size % 16:
             raise ValueError("block_size must be a multiple of 16")
         _check_choice("tp_comm", self.tp_comm, ("fused", "nccl"))
+        _check_choice("kv_cache_dtype", self.kv_cache_dtype, ("auto", "int4"))
+        if self.kv_cache_group not in (32, 64, 128):
+            raise ValueError("kv_cache_group must be 32, 64 or 128")
         if self.max_lora_rank % 8:
             raise ValueError("max_lora_rank must be a multiple of 8")
 

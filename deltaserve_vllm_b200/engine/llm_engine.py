@@ -262,8 +262,11 @@ class CoServingEngine:
     def _alloc_kv(self) -> KVCache:
         e = self.ecfg
         hkv = self.arch.num_kv_heads // self.tp.size
+        group = e.kv_cache_group if e.kv_cache_dtype == "int4" else None
+        if group and (self.arch.head_dim != 128 or self.arch.num_heads // self.arch.num_kv_heads > 16):
+            raise ValueError("kv_cache_dtype int4 needs head_dim 128 and at most 16 query heads per KV head")
         per_block = KVCache.bytes_per_block(self.arch.num_layers, hkv, e.block_size,
-                                            self.arch.head_dim, 2 if self.cuda else 4)
+                                            self.arch.head_dim, 2 if self.cuda else 4, group)
         if e.num_gpu_blocks_override:
             nb = e.num_gpu_blocks_override
         elif self.cuda:
@@ -281,7 +284,7 @@ class CoServingEngine:
         if nb < 2:
             raise MemoryError("no room for the KV cache")
         return KVCache(self.arch.num_layers, nb, hkv, e.block_size, self.arch.head_dim, self.device,
-                       self.dtype, prefix_caching=e.enable_prefix_caching)
+                       self.dtype, prefix_caching=e.enable_prefix_caching, kv_group=group)
 
     def _check_stop_strings(self, out, now: float) -> list:
         """Requests whose decoded output now contains one of their stop strings."""
@@ -608,6 +611,41 @@ class CoServingEngine:
         for cb in self.request_listeners:
             cb("add", r)
         return r
+
+    def fork_request(self, request_id: str, new_id: str, params: SamplingParams | None = None) -> Request:
+        """A copy of a decoding request that goes on by itself from the same
+        tokens (with ``params``, e.g. another seed): full KV pages are shared,
+        the partly filled one is copied. Single rank only."""
+        if self.tp_size > 1:
+            raise ValueError("fork_request needs tensor_parallel_size 1")
+        if new_id in self.requests:
+            raise ValueError(f"request {new_id!r} exists")
+        r = self.requests.get(request_id)
+        if r is None or r not in self.scheduler.running or r.in_prefill:
+            raise KeyError(f"no decoding request {request_id!r}")
+        if len(self.scheduler.running) >= self.ecfg.max_num_seqs:
+            raise MemoryError("max_num_seqs requests are running")
+        child = Request(new_id, list(r.prompt_ids), params or r.params, r.adapter, status=r.status,
+                        output_ids=list(r.output_ids), num_computed=r.num_computed, lora_slot=r.lora_slot,
+                        num_cached_tokens=r.num_computed, first_token_time=r.first_token_time,
+                        block_hashes=list(r.block_hashes))
+        child.output_logprobs = list(r.output_logprobs)
+        child.output_top_logprobs = list(r.output_top_logprobs)
+        child.block_ids = self.kv.fork([(r.block_ids, r.num_computed)])[0]
+        child.num_registered = min(r.num_registered, r.num_computed // self.kv.block_size)
+        self.scheduler.running.append(child)
+        self.requests[new_id] = child
+        for cb in self.request_listeners:
+            cb("add", child)
+        return child
+
+    def compact_kv(self) -> int:
+        """Move the KV pages in use to the front of the pool (between steps).
+        Returns how many are in use. Single rank only."""
+        if self.tp_size > 1:
+            raise ValueError("compact_kv needs tensor_parallel_size 1")
+        held = list(self.scheduler.running) + list(self.scheduler.waiting)
+        return self.kv.compact([r.block_ids for r in held])
 
     def abort_request(self, request_id: str) -> bool:
         if self.router is not None and self.router.cancel(request_id):

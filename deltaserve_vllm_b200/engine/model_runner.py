@@ -286,7 +286,7 @@ class ModelRunner:
                        if (decode_graphs and self.device.type == "cuda") else None)
 
     def graph_eligible(self, meta: dict) -> bool:
-        return (self.graphs is not None and meta["npf"] == 0 and meta["nd"] > 0
+        return (self.graphs is not None and meta["npf"] == 0 and meta["ft_rows"] == 0 and meta["nd"] > 0
                 and not meta.get("full_sampler", False)
                 and DecodeGraphs.bucket(meta["nd"]) is not None)
 
@@ -373,7 +373,13 @@ class ModelRunner:
             pk.add("dec_ctx", ctx)
             hkv = self.model.hkv_l
             splits, kps = ops.decode_splits(nd, hkv, max(ctx), self.num_sms)
-        pf = out.prefill + out.ft
+        # Over a 4-bit cache FT samples attend to their own rows (their own tile list).
+        own_rows = self.model.kv4 and bool(out.ft)
+        pf = out.prefill if own_rows else out.prefill + out.ft
+        if own_rows:
+            lens = [s.num_new for s in out.ft]
+            starts = np.cumsum([0] + lens[:-1]).tolist()
+            pk.add("ft_tiles", ops.dense_attn_tiles(starts, lens, "cpu", bm=128).numpy().reshape(-1))
         if pf:
             btab = np.zeros((len(pf), maxb), dtype=np.int64)
             cu = [0]
@@ -404,7 +410,7 @@ class ModelRunner:
         pk.add("logits_idx", sample_rows)
         meta = {"full_sampler": any(r.params.needs_full_sampler for r in sample_reqs),
                 "nd": nd, "maxb": maxb, "splits": splits, "kps": kps, "npf": len(pf),
-                "use_lora": use_lora, "T": T, "ft_rows": sum(s.num_new for s in out.ft),
+                "own_rows": own_rows, "use_lora": use_lora, "T": T, "ft_rows": sum(s.num_new for s in out.ft),
                 "ft_dst": ft_dst}
         return meta, pk, sample_reqs
 
@@ -431,6 +437,7 @@ class ModelRunner:
             pf_ctx_lens=i32(d["pf_ctx"]) if pf else None,
             pf_block_tables=i32(d["pf_btab"]).view(pf, maxb) if pf else None,
             pf_tile_info=i32(d["pf_tiles"]).view(-1, 2) if pf else None,
+            ft_attn_tiles=i32(d["ft_tiles"]).view(-1, 3) if meta["own_rows"] else None,
             slot_ids=i32(d["lslot"]) if use_lora else None,
             tile_slots=i32(d["tile_slots"]) if use_lora else None,
             logits_idx=d["logits_idx"],

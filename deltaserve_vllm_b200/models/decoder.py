@@ -58,6 +58,9 @@ class ForwardBatch:
     pf_ctx_lens: torch.Tensor | None = None        # [S] int32
     pf_block_tables: torch.Tensor | None = None    # [S, maxb] int32
     pf_tile_info: torch.Tensor | None = None       # [tiles, 2] int32
+    # 4-bit cache: FT samples attend to their own rows, not to the cache. The
+    # prefill fields then hold the inference sequences only.
+    ft_attn_tiles: torch.Tensor | None = None      # [tiles, 3] int32, rows relative to ft_lo
     slot_ids: torch.Tensor | None = None           # [T] int32 LoRA slot per token (-1 none)
     tile_slots: torch.Tensor | None = None         # [ceil(T/128)] int32 slot bitmask per M tile
     logits_idx: torch.Tensor | None = None         # [R] int64 rows whose logits are needed
@@ -130,6 +133,8 @@ class DecoderModel:
         self.w = weights
         self.arch: ModelArch = weights.arch
         self.kv_k, self.kv_v = kv_k, kv_v
+        # A 4-bit cache is one uint8 tensor per layer (K and V) in ``kv_k``.
+        self.kv4 = bool(kv_k) and kv_k[0].dtype == torch.uint8
         self.lora = lora
         self.comm = comm or Communicator()
         dev = weights.embed.device
@@ -140,6 +145,7 @@ class DecoderModel:
         self.hkv_l = self.arch.num_kv_heads // weights.tp.size
         self.scale = 1.0 / math.sqrt(self.arch.head_dim)
         self._dec_ws: tuple[torch.Tensor, torch.Tensor] | None = None
+        self._kv4_ws = ops.kv4_workspace(dev) if self.kv4 else None
         # A parallel.peer.PeerTable of the embedding shards (set by the engine
         # under TP with the fused communication path) replaces embedding + all-reduce.
         self.embed_peer = None
@@ -186,6 +192,8 @@ class DecoderModel:
 
     def attention(self, layer: int, qkv: torch.Tensor, ctx: torch.Tensor, b: ForwardBatch):
         q = qkv[:, : self.w.q_local]
+        if self.kv4:
+            return self._attention4(layer, qkv, q, ctx, b)
         kc, vc = self.kv_k[layer], self.kv_v[layer]
         nd = b.num_decode
         if nd > 0:
@@ -195,6 +203,23 @@ class DecoderModel:
         if b.num_prefill_seqs > 0:
             ops.paged_prefill(q[nd:], kc, vc, b.pf_block_tables, b.pf_cu_q, b.pf_ctx_lens,
                               b.pf_tile_info, ctx[nd:], self.hq_l, self.scale)
+
+    def _attention4(self, layer: int, qkv: torch.Tensor, q: torch.Tensor, ctx: torch.Tensor, b: ForwardBatch):
+        """Attention over a 4-bit cache. FT rows (whole samples) attend to their
+        unquantised rows: the LoRA backward differentiates exactly that."""
+        nd, cache = b.num_decode, self.kv_k[layer]
+        hi = b.ft_lo if b.ft_attn_tiles is not None else q.shape[0]
+        if nd > 0:
+            ops.paged_decode4(q[:nd], cache, b.dec_block_tables, b.dec_ctx_lens, ctx[:nd], self.hq_l, self.scale,
+                              self._kv4_ws)
+        if b.num_prefill_seqs > 0:
+            ops.paged_prefill4(q[nd:hi], cache, b.pf_block_tables, b.pf_cu_q, b.pf_ctx_lens, ctx[nd:hi], self.hq_l,
+                               self.scale, self._kv4_ws)
+        if b.ft_attn_tiles is not None:
+            rows = qkv[hi:].unflatten(1, (-1, self.arch.head_dim))
+            k0, v0 = self.hq_l, self.hq_l + self.hkv_l
+            ops.attn_fwd_dense(rows[:, :k0], rows[:, k0:v0], rows[:, v0:], None, self.scale, ctx[hi:],
+                               tiles128=b.ft_attn_tiles)
 
     # ------------------------------------------------------------------ forward
     @torch.no_grad()
@@ -238,8 +263,14 @@ class DecoderModel:
             self._proj(x, lw.qkv, qkv, l, "qkv", b,
                        save=cap.qkv[l] if cap_on and cap.qkv is not None else None,
                        save_lo=lo, save_hi=hi, save_dst=dst)
-            ops.qk_norm_rope_cache(qkv, b.positions, self.cos_sin, lw.q_norm, lw.k_norm, eps,
-                                   self.hq_l, self.hkv_l, self.kv_k[l], self.kv_v[l], b.slot_mapping)
+            if self.kv4:
+                ops.qk_norm_rope_cache(qkv, b.positions, self.cos_sin, lw.q_norm, lw.k_norm, eps,
+                                       self.hq_l, self.hkv_l)
+                ops.kv4_write(qkv[:, w.q_local:w.q_local + w.kv_local], qkv[:, w.q_local + w.kv_local:],
+                              self.kv_k[l], b.slot_mapping)
+            else:
+                ops.qk_norm_rope_cache(qkv, b.positions, self.cos_sin, lw.q_norm, lw.k_norm, eps,
+                                       self.hq_l, self.hkv_l, self.kv_k[l], self.kv_v[l], b.slot_mapping)
             self.attention(l, qkv, ctx, b)
             if cap_on and cap.ctx is not None:
                 cap.ctx[l, dst:dst + hi - lo] = ctx[lo:hi]
