@@ -170,3 +170,11 @@ def test_configuration_refusals():
         KVCache(1, 2, 1, 16, 64, "cpu", kv_group=64)
     with pytest.raises(ValueError):
         ops.kv4_cache_shape(1, 1, 8, 64)
+
+
+def test_comparison_command_runs():
+    from deltaserve_vllm_b200.eval.kv4_compare import main
+    res = main(["--model", "llama3-test", "--batch", "2", "--prompt", "40", "--tokens", "8", "--device", "cpu",
+                "--blocks", "16"])
+    assert res["int4"]["page_bytes"] * 2 * 256 == res["auto"]["page_bytes"] * 72      # fp32 pages on CPU
+    assert res["int4"]["fork"]["same_tokens"]

@@ -1,0 +1,112 @@
+"""Serving over a 4-bit KV cache on the GPU: against the CPU path, with CUDA
+graphs, co-serving with finetuning, and with forked requests."""
+import pytest
+import torch
+
+from deltaserve_vllm_b200 import ops
+from deltaserve_vllm_b200.config import EngineConfig, FinetuneConfig
+from deltaserve_vllm_b200.engine.ft.store import FinetuningStore
+from deltaserve_vllm_b200.engine.kv_cache import KVCache
+from deltaserve_vllm_b200.engine.llm_engine import CoServingEngine
+from deltaserve_vllm_b200.engine.model_runner import ModelRunner
+from deltaserve_vllm_b200.engine.request import Request, SamplingParams
+from deltaserve_vllm_b200.engine.scheduler import Scheduler
+from deltaserve_vllm_b200.models.configs import PRESETS
+from deltaserve_vllm_b200.models.decoder import DecoderModel
+from deltaserve_vllm_b200.models.weights import init_weights
+
+pytestmark = pytest.mark.gpu
+
+
+def run(name, dev, dt, forced=None, graphs=False):
+    arch = PRESETS[name]
+    w = init_weights(arch, seed=11, device="cpu", dtype=torch.float32).to(dev, dt)
+    kv = KVCache(arch.num_layers, 32, arch.num_kv_heads, 64, 128, dev, dt, kv_group=64)
+    sched = Scheduler(kv.allocator, 64, max_num_batched_tokens=160, max_model_len=1024)
+    runner = ModelRunner(DecoderModel(w, kv.k, kv.v, None), 64, dev, max_model_len=1024, decode_graphs=graphs)
+    g = torch.Generator().manual_seed(0)
+    for i, n in enumerate([200, 37, 1, 130]):
+        sched.add(Request(str(i), torch.randint(0, arch.vocab, (n,), generator=g).tolist(), SamplingParams(max_tokens=4)))
+    logits_all, toks_all = [], []
+    for step in range(20):
+        out = sched.schedule()
+        if out.is_empty():
+            break
+        toks, logits = runner.execute(out)
+        by_rid = {s.req.request_id: toks[s.req.seq_no] for s in out.seqs if s.req.seq_no in toks}
+        if forced is not None:
+            by_rid = forced[step]
+            toks = {s.req.seq_no: by_rid[s.req.request_id] for s in out.seqs if s.req.request_id in by_rid}
+        toks_all.append(by_rid)
+        logits_all.append(None if logits is None else logits.float().cpu().clone())
+        sched.update(out, toks)
+    if dev == "cuda":
+        assert ops.check_device_error() == 0
+    return logits_all, toks_all, runner
+
+
+@pytest.mark.parametrize("name", ["qwen3-test", "llama3-test"])
+def test_gpu_matches_cpu(name):
+    """bf16 activations move some codes by a step: the two runs differ by less
+    than quantisation itself does (a third of the logits' spread at most)."""
+    cpu, toks, _ = run(name, "cpu", torch.float32)
+    gpu, _, _ = run(name, "cuda", torch.bfloat16, forced=toks)
+    assert len(cpu) == len(gpu)
+    for a, b in zip(gpu, cpu):
+        if a is not None and a.numel():
+            assert float((a - b).norm() / (b - b.mean()).norm()) < 1 / 3
+
+
+@pytest.mark.parametrize("name", ["qwen3-test", "llama3-test"])
+def test_decode_graphs_match_eager(name):
+    _, toks, _ = run(name, "cpu", torch.float32)
+    eager, _, _ = run(name, "cuda", torch.bfloat16, forced=toks)
+    graph, _, runner = run(name, "cuda", torch.bfloat16, forced=toks, graphs=True)
+    assert runner.graphs.replays > 0
+    for a, b in zip(eager, graph):
+        if a is not None and a.numel():
+            torch.testing.assert_close(b, a, rtol=2e-2, atol=5e-2)
+
+
+def test_coserving_over_a_4_bit_cache():
+    ecfg = EngineConfig(model="qwen3-test", max_model_len=1024, block_size=64, max_num_batched_tokens=2048, max_loras=2,
+                        max_lora_rank=16, num_gpu_blocks_override=256, kv_cache_dtype="int4",
+                        enable_prefix_caching=True)
+    fcfg = FinetuneConfig(enable_finetuning=True, backward_cuda_graph=True, max_saved_finetuning_tokens=512,
+                          learning_rate=1e-3)
+    store = FinetuningStore.synthetic(4096, 40, 64, 128, seed=0, max_saved_finetuning_tokens=512, total_epochs=2)
+    eng = CoServingEngine(ecfg, fcfg, ft_store=store)
+    eng.load_inference_adapter("inf", rank=16, alpha=32)
+    g = torch.Generator().manual_seed(0)
+    for i in range(12):
+        eng.add_request(f"r{i}", torch.randint(0, 4096, (50 + 30 * i,), generator=g).tolist(),
+                        SamplingParams(max_tokens=8), adapter="inf" if i % 2 else None)
+    eng.run_until_idle(max_steps=5000)
+    eng.synchronize()
+    assert ops.check_device_error() == 0
+    assert eng.coord.completed_cycles >= 4, eng.finetuning_status()
+    assert all(l == l and l > 0 for l in eng.trainer.losses)
+    assert len([r for r in eng.finished if r.request_id.startswith("r")]) == 12
+    assert eng.kv.allocator.num_free == eng.kv.allocator.num_blocks
+
+
+@pytest.mark.parametrize("dtype", ["int4", "auto"])
+def test_fork_and_compact(dtype):
+    """A greedy fork repeats its parent, and compaction between steps changes nothing."""
+    ecfg = EngineConfig(model="llama3-test", max_model_len=1024, block_size=64, max_num_batched_tokens=2048, max_loras=2,
+                        max_lora_rank=16, num_gpu_blocks_override=64, kv_cache_dtype=dtype)
+    eng = CoServingEngine(ecfg, FinetuneConfig(enable_finetuning=False))
+    g = torch.Generator().manual_seed(2)
+    for i, n in enumerate((100, 300, 70)):
+        eng.add_request(f"r{i}", torch.randint(0, 4096, (n,), generator=g).tolist(),
+                        SamplingParams(max_tokens=20 if i else 2))
+    while len(eng.requests["r2"].output_ids) < 4:
+        eng.step()
+    eng.fork_request("r2", "fork")
+    used = eng.compact_kv()
+    assert max(p for r in eng.scheduler.running for p in r.block_ids) < used
+    eng.run_until_idle(max_steps=500)
+    assert ops.check_device_error() == 0
+    got = {r.request_id: r.output_ids for r in eng.finished}
+    assert got["fork"] == got["r2"] and len(got["r1"]) == 20
+    assert eng.kv.allocator.num_free == eng.kv.allocator.num_blocks

@@ -72,6 +72,34 @@ def test_write_and_read_match_the_format(n, hkv, page, group, start):
     assert torch.equal(gk.cpu(), ek) and torch.equal(gv.cpu(), ev)
 
 
+@pytest.mark.parametrize("group", ops.KV4_GROUPS)
+@pytest.mark.parametrize("start", [0, 3, 15])
+@pytest.mark.parametrize("kind", ["sequences", "holes", "shuffled", "repeats_a_page"])
+def test_many_rows_fill_whole_records_or_not(kind, start, group):
+    """Enough rows that 16 of them go together where they fill a record: sequences that begin anywhere,
+    -1 slots inside, unordered slots, records that are full in the cache but not by rows that follow one another."""
+    g = gen(4 + start)
+    n, hkv, page = 1100, 8, 48
+    k, v = rows(g, n, hkv).flatten(1), rows(g, n, hkv).flatten(1)
+    slots = torch.cat([torch.arange(m, device=DEV) + 48 * 13 * i + (start if i % 2 else 0) for i, m in
+                       enumerate([600, 37, 16, 15, 432])])
+    pages = 13 * 5
+    if kind == "holes":
+        slots[5::61] = -1
+    elif kind == "shuffled":
+        slots = slots[torch.randperm(n, generator=g, device=DEV)]
+    elif kind == "repeats_a_page":
+        slots = slots.view(-1, 2).flip(1).flatten().clone()
+    got = empty_cache(pages, hkv, page, group)
+    ops.kv4_write(k, v, got, slots)
+    exp = empty_cache(pages, hkv, page, group)
+    for i in range(0, n, 100):               # few rows at a time: one by one
+        ops.kv4_write(k[i:i + 100], v[i:i + 100], exp, slots[i:i + 100])
+    assert torch.equal(got, exp)
+    assert torch.equal(ops.kv4_read(got, slots)[0], torch.cat([ops.kv4_read(got, s)[0] for s in slots.split(100)]))
+    assert torch.equal(ops.kv4_read(got, slots)[1], torch.cat([ops.kv4_read(got, s)[1] for s in slots.split(100)]))
+
+
 @pytest.mark.parametrize("order", ["shuffled", "reversed", "two_runs"])
 def test_write_takes_slots_in_any_order(order):
     """Slots that do not follow one another, or do so only for a part of a 16-token record."""
