@@ -10,6 +10,10 @@
 
 namespace dsv {
 
+// Rows x heads from which records are assembled (rows of 8 heads, one by one
+// against by records: 2048 rows 9.4 / 11.5 us, 8192 rows 31.5 / 25.1 us).
+constexpr int64_t KV4_MANY = 32768;
+
 struct Kv4RowsArgs {
   const __nv_bfloat16* k;   // [T, Hkv, 128], strides in elements
   const __nv_bfloat16* v;
@@ -42,14 +46,15 @@ __device__ __forceinline__ float nan_max(float a, float b) {
   return d;
 }
 
-// Quantise this lane's 4 channels (4 lane .. + 3) of a row; the group's
-// statistics come from the 32 / NG lanes that share it. Returns the four codes
-// as nibbles and the group's (scale, zero) word. Each step is rounded as the
-// format says (no contraction), so any implementation of it gives these bits.
+// Quantising this lane's 4 channels (4 lane .. + 3) of a row, in three steps.
+// Each is rounded as the format says (no contraction), so any implementation of
+// it gives these bits.
+//
+// The group's range; the 32 / NG lanes that share the group all get it.
 template <int NG>
-__device__ __forceinline__ uint32_t kv4_quantise(float (&x)[4], uint32_t& word) {
-  float lo = nan_min(nan_min(x[0], x[1]), nan_min(x[2], x[3]));
-  float hi = nan_max(nan_max(x[0], x[1]), nan_max(x[2], x[3]));
+__device__ __forceinline__ void kv4_range(float (&x)[4], float& lo, float& hi) {
+  lo = nan_min(nan_min(x[0], x[1]), nan_min(x[2], x[3]));
+  hi = nan_max(nan_max(x[0], x[1]), nan_max(x[2], x[3]));
   if (__any_sync(0xffffffffu, !(lo >= -KV4_LIMIT && hi <= KV4_LIMIT))) {       // saturate; a NaN counts as 0
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = x[e] == x[e] ? fminf(fmaxf(x[e], -KV4_LIMIT), KV4_LIMIT) : 0.f;
@@ -63,14 +68,18 @@ __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[4], uint32_t& word) 
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
+}
+// Its (scale, zero point) word and the scale's reciprocal.
+__device__ __forceinline__ uint32_t kv4_word(float lo, float hi, float& inv) {
   float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
   if (s < KV4_TINY) s = 0.f;
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  const __half zh = __float2half_rn(__fmul_rn(lo, inv));
-  const float z = __half2float(zh);
-  word = __float_as_uint(s) | __half_as_ushort(zh);
-  // In [0, 15] adding 1.5 * 2^23 rounds to the nearest integer (ties to even)
-  // and leaves it in the low bits.
+  inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  return __float_as_uint(s) | __half_as_ushort(__float2half_rn(__fmul_rn(lo, inv)));
+}
+// The four codes as nibbles. In [0, 15] adding 1.5 * 2^23 rounds to the nearest
+// integer (ties to even) and leaves it in the low bits.
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[4], uint32_t word, float inv) {
+  const float z = kv4_zero(word);
   uint32_t u[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -96,25 +105,29 @@ __device__ __forceinline__ void kv4_load4(const __nv_bfloat16* p, bool vec, floa
   }
 }
 
-// Quantise a row's K and V of one head into token r of a record (K's part at
-// `krec`, shared or global memory): one warp, lane owns 4 channels.
+// This lane's 4 channels of a row's K and V of one head.
+__device__ __forceinline__ void kv4_load_row(const Kv4RowsArgs& a, bool vec, int row, int head, float (&x)[4],
+                                             float (&y)[4]) {
+  const int c = 4 * (threadIdx.x & 31);
+  kv4_load4(a.k + row * a.k_row + head * a.k_head + c, vec, x);
+  kv4_load4(a.v + row * a.v_row + head * a.v_head + c, vec, y);
+}
+
+// Codes and word of token r of a record's K or V part (shared or global memory).
 template <int NG>
-__device__ __forceinline__ void kv4_put_row(const Kv4RowsArgs& a, bool vec, int row, int head, uint8_t* krec, int r) {
+__device__ __forceinline__ void kv4_put_k(uint8_t* krec, int r, uint32_t c, uint32_t word) {
   const int lane = threadIdx.x & 31;
-  uint8_t* vrec = krec + kv4_record(NG);
-  float x[4], y[4];
-  kv4_load4(a.k + row * a.k_row + head * a.k_head + 4 * lane, vec, x);
-  kv4_load4(a.v + row * a.v_row + head * a.v_head + 4 * lane, vec, y);
-  uint32_t word;
-  uint32_t c = kv4_quantise<NG>(x, word);
-  // K: lane's codes are half a word of channels 32 i + 8 t + 0..7
+  // lane's codes are half a word of channels 32 i + 8 t + 0..7
   const uint32_t up = __shfl_down_sync(0xffffffffu, c, 1);
   if (!(lane & 1))
     *reinterpret_cast<uint32_t*>(krec + 64 * r + 16 * (lane % 8 / 2) + 4 * (lane / 8)) = c | up << 16;
   if (lane % (32 / NG) == 0)
     *reinterpret_cast<uint32_t*>(krec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r) = word;
-  c = kv4_quantise<NG>(y, word);
-  // V: channels g and g + 8 of a 16-channel tile share a byte; lane ^ 2 holds the other half
+}
+template <int NG>
+__device__ __forceinline__ void kv4_put_v(uint8_t* vrec, int r, uint32_t c, uint32_t word) {
+  const int lane = threadIdx.x & 31;
+  // channels g and g + 8 of a 16-channel tile share a byte; lane ^ 2 holds the other half
   const uint32_t hi = __shfl_down_sync(0xffffffffu, c, 2);
   if (!(lane & 2)) {
     uint8_t* dst = vrec + 512 * (lane / 16) + 16 * (r % 8 / 2) + 4 * (lane / 4 % 4) + (r / 8) + 2 * (r % 2);
@@ -124,6 +137,50 @@ __device__ __forceinline__ void kv4_put_row(const Kv4RowsArgs& a, bool vec, int 
   }
   if (lane % (32 / NG) == 0)
     *reinterpret_cast<uint32_t*>(vrec + KV4_CODES + 64 * (lane * NG / 32) + 4 * r) = word;
+}
+
+// One row's K and V into token r of the record at `krec`.
+template <int NG>
+__device__ __forceinline__ void kv4_put_row(float (&x)[4], float (&y)[4], uint8_t* krec, int r) {
+  float lo, hi, inv;
+  kv4_range<NG>(x, lo, hi);
+  uint32_t word = kv4_word(lo, hi, inv);
+  kv4_put_k<NG>(krec, r, kv4_codes(x, word, inv), word);
+  kv4_range<NG>(y, lo, hi);
+  word = kv4_word(lo, hi, inv);
+  kv4_put_v<NG>(krec + kv4_record(NG), r, kv4_codes(y, word, inv), word);
+}
+
+// Four rows' words at once: their 8 NG groups (K and V) take one lane each, so
+// that the two exact divisions run once and not eight times. put(j, c, word,
+// d, word) stores row j's K and V.
+template <int NG, class Put>
+__device__ __forceinline__ void kv4_four_rows(float (&x)[4][4], float (&y)[4][4], Put put) {
+  const int lane = threadIdx.x & 31;
+  float lo[8], hi[8], mylo = 0.f, myhi = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    kv4_range<NG>(x[j], lo[2 * j], hi[2 * j]);
+    kv4_range<NG>(y[j], lo[2 * j + 1], hi[2 * j + 1]);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {                // lane 8 i + k takes group i of item k
+    const float a = __shfl_sync(0xffffffffu, lo[k], (lane >> 3) % NG * (32 / NG));
+    const float b = __shfl_sync(0xffffffffu, hi[k], (lane >> 3) % NG * (32 / NG));
+    if ((lane & 7) == k) {
+      mylo = a;
+      myhi = b;
+    }
+  }
+  float inv;
+  const uint32_t word = kv4_word(mylo, myhi, inv);
+  const int from = 8 * (lane * NG / 32);       // this lane's own group
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t kw = __shfl_sync(0xffffffffu, word, from + 2 * j), vw = __shfl_sync(0xffffffffu, word, from + 2 * j + 1);
+    const float ki = __shfl_sync(0xffffffffu, inv, from + 2 * j), vi = __shfl_sync(0xffffffffu, inv, from + 2 * j + 1);
+    put(j, kv4_codes(x[j], kw, ki), kw, kv4_codes(y[j], vw, vi), vw);
+  }
 }
 
 // The values of token r of a record (null: zeros) as bf16 rows.
@@ -155,12 +212,9 @@ __device__ __forceinline__ void kv4_get_row(const Kv4RowsArgs& a, int row, int h
   *reinterpret_cast<uint2*>(a.v_out + at) = vo;
 }
 
-// One warp = one (row, head), K and V. Bound by instructions until their count was
-// halved (rounding by an addition, the odd inputs in a branch of their own); now
-// 8192 rows of 8 heads are @W us (write) and @R us (read back) against 6.6 us of
-// HBM. Assembling whole records of 16 rows in shared memory first (one run of
-// 16-byte stores in place of a token's 64 single bytes) measured slower: 41 against
-// 32 us at that size, 35 against 6 us at 1024 rows.
+// One warp = one (row, head), K and V: 64 rows of 8 heads are written in 2.8 us
+// and read in 2.3 us, 8192 read in 18 us (6.6 us of HBM bytes; the single-byte
+// V accesses and their partial sectors are what it waits for).
 template <int NG, bool WRITE>
 __global__ void __launch_bounds__(256) kv4_row_kernel(const Kv4RowsArgs a, bool vec) {
   const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 32;
@@ -174,15 +228,98 @@ __global__ void __launch_bounds__(256) kv4_row_kernel(const Kv4RowsArgs a, bool 
   int r = 0;
   uint8_t* krec = slot >= 0 ? kv4_record_of<NG>(a, slot, head, r) : nullptr;
   if (!WRITE) kv4_get_row<NG>(a, row, head, krec, r);
-  else if (krec != nullptr) kv4_put_row<NG>(a, vec, row, head, krec, r);
+  else if (krec != nullptr) {
+    float x[4], y[4];
+    kv4_load_row(a, vec, row, head, x, y);
+    kv4_put_row<NG>(x, y, krec, r);
+  }
+}
+
+// Writing many rows: four warps = 16 rows of one head. Where 16 rows that follow
+// one another fill a record (most of a prompt), the record is assembled in
+// shared memory and stored as one run of 16-byte accesses: a lone token's V codes
+// are 64 bytes in 16 sectors, and those partial sectors bound the row-by-row
+// kernel (32 us for 8192 rows of 8 heads, whatever its instruction count). The
+// record belongs to the warps whose rows it begins in; rows outside such records
+// go one by one. A row's quantisation is a chain of about a microsecond (two
+// statistics across lanes, two exact divisions): hence four rows per warp, whose
+// divisions share a pass. 8192 rows of 8 heads: 25 us (16 rows per warp: 36 us).
+template <int NG>
+__global__ void __launch_bounds__(256) kv4_write_records_kernel(const Kv4RowsArgs a, bool vec) {
+  constexpr int REC = 2 * kv4_record(NG);
+  __shared__ __align__(16) uint8_t records[2][REC];
+  const int lane = threadIdx.x & 31, team = threadIdx.x / 128, part = threadIdx.x / 32 & 3;
+  uint8_t* rec = records[team];
+  const int64_t w = (int64_t)blockIdx.x * 2 + team;
+  const int head = (int)(w % a.heads), row0 = (int)(w / a.heads) * 16;
+  if (row0 >= a.rows) return;                 // the whole team
+  // Window of 48 rows from 16 before ours: bit j of `run`: row j + 1's slot is
+  // the next one; of `begins`: row j's slot begins a record that 16 rows fill.
+  auto slot_of = [&](int row) { return row >= 0 && row < a.rows ? a.slots[row] : (int64_t)-1; };
+  const int64_t s0 = slot_of(row0 - 16 + lane), s1 = slot_of(row0 + 16 + lane);
+  const int64_t n0 = __shfl_down_sync(0xffffffffu, s0, 1), n1 = __shfl_down_sync(0xffffffffu, s1, 1);
+  const int64_t first1 = __shfl_sync(0xffffffffu, s1, 0);
+  const bool f0 = s0 >= 0 && (lane == 31 ? first1 : n0) == s0 + 1, f1 = s1 >= 0 && lane < 31 && n1 == s1 + 1;
+  const bool b0 = s0 >= 0 && (s0 & 15) == 0 && s0 + 15 < a.num_slots;
+  const bool b1 = s1 >= 0 && (s1 & 15) == 0 && s1 + 15 < a.num_slots;
+  uint64_t run = __ballot_sync(0xffffffffu, f0) | (uint64_t)__ballot_sync(0xffffffffu, f1) << 32;
+  run &= run >> 1;
+  run &= run >> 2;
+  run &= run >> 4;                            // eight steps in a row
+  run &= run >> 7;                            // fifteen
+  const uint64_t begins = run & (__ballot_sync(0xffffffffu, b0) | (uint64_t)__ballot_sync(0xffffffffu, b1) << 32);
+  uint64_t whole = begins;                    // rows of whole records
+  whole |= whole << 1;
+  whole |= whole << 2;
+  whole |= whole << 4;
+  whole |= whole << 8;
+  const uint32_t mine = (uint32_t)(begins >> 16) & 0xffffu;
+  if (mine != 0) {
+    const int row = row0 + __ffs(mine) - 1;
+    int r;
+    uint8_t* dst = kv4_record_of<NG>(a, a.slots[row], head, r);
+    float x[4][4], y[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kv4_load_row(a, vec, row + 4 * part + j, head, x[j], y[j]);
+    kv4_four_rows<NG>(x, y, [&](int j, uint32_t kc, uint32_t kw, uint32_t vc, uint32_t vw) {
+      kv4_put_k<NG>(rec, 4 * part + j, kc, kw);
+      kv4_put_v<NG>(rec + kv4_record(NG), 4 * part + j, vc, vw);
+    });
+    named_bar_sync(1 + team, 128);
+    for (int i = threadIdx.x & 127; i < REC / 16; i += 128)
+      reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(rec)[i];
+  }
+  // The rest of this warp's four rows.
+  const bool own = lane < 16 ? false : s0 >= 0 && !(whole >> lane & 1u);       // window rows 16..31 are ours
+  if (own && s0 >= a.num_slots) set_error(kErrShape);
+  const uint32_t rest = __ballot_sync(0xffffffffu, own && s0 < a.num_slots) >> 16;
+  if (!(rest >> (4 * part) & 15u)) return;
+  float x[4][4], y[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) kv4_load_row(a, vec, min(row0 + 4 * part + j, a.rows - 1), head, x[j], y[j]);
+  kv4_four_rows<NG>(x, y, [&](int j, uint32_t kc, uint32_t kw, uint32_t vc, uint32_t vw) {
+    const int64_t slot = __shfl_sync(0xffffffffu, s0, 16 + 4 * part + j);
+    if (!(rest >> (4 * part + j) & 1u)) return;
+    int r;
+    uint8_t* krec = kv4_record_of<NG>(a, slot, head, r);
+    kv4_put_k<NG>(krec, r, kc, kw);
+    kv4_put_v<NG>(krec + kv4_record(NG), r, vc, vw);
+  });
 }
 
 template <bool WRITE>
 static void kv4_rows_launch(const Kv4RowsArgs& a, bool vec, int ng) {
-  const int64_t blocks = ((int64_t)a.rows * a.heads + 7) / 8;
-  if (blocks == 0) return;
-  auto kernel = ng == 1 ? kv4_row_kernel<1, WRITE> : ng == 2 ? kv4_row_kernel<2, WRITE> : kv4_row_kernel<4, WRITE>;
-  kernel<<<(unsigned)blocks, 256, 0, at::cuda::getCurrentCUDAStream()>>>(a, vec);
+  if (a.rows == 0) return;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  if (WRITE && (int64_t)a.rows * a.heads >= KV4_MANY) {
+    const int64_t teams = (int64_t)((a.rows + 15) / 16) * a.heads;
+    auto kernel = ng == 1 ? kv4_write_records_kernel<1> : ng == 2 ? kv4_write_records_kernel<2> : kv4_write_records_kernel<4>;
+    kernel<<<(unsigned)((teams + 1) / 2), 256, 0, stream>>>(a, vec);
+  } else {
+    const int64_t warps = (int64_t)a.rows * a.heads;
+    auto kernel = ng == 1 ? kv4_row_kernel<1, WRITE> : ng == 2 ? kv4_row_kernel<2, WRITE> : kv4_row_kernel<4, WRITE>;
+    kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(a, vec);
+  }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

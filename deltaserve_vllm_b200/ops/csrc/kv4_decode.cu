@@ -17,6 +17,14 @@
 // them: by eights, in a tree over the runs' numbers, so that a context spread
 // over the whole GPU takes four short joins and the result does not depend on
 // the order of arrival.
+//
+// Measured against the HBM time of the cache bytes (6.54 TB/s): batch 200 x 4096,
+// 32 / 8 heads, groups of 64: 176 us, 5.4 TB/s (one record per step in place of
+// two: 4.5); 16 x 32768, 64 / 8 heads: 125 us. There about 260 instructions per
+// 16 tokens and their latencies bound it (issue slots 56 % busy, ALU 51 %). Short
+// contexts are bound by a segment's fixed chain of about 2 us (queries, last
+// partial sums, store) and a join's 3 us (release, counter, two rounds of loads).
+// At least two pieces a run: 1 measured 9.9, 2 7.6 and 4 10.5 us at 64 x 64 tokens.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -20,8 +20,8 @@
 //                    from TMEM. Tile 0's softmax runs while tile 1's products do.
 //
 // Operands are fp16 (fp32 accumulators): a value s (c + z) of the 4-bit format
-// fits 11 bits to within 2^-12 of its group's range, where bf16 would double the
-// result's own rounding error. K's and V's values stay below 8704 and P below
+// fits its 11 bits to within 2^-12 of itself, where bf16 operands would double the
+// result's own rounding error. K and V enter divided by 16 (below 545) and P below
 // 2^8; each query row is scaled by a power of two (its largest magnitude lands
 // in [1, 2)), which the softmax undoes.
 //
@@ -33,6 +33,12 @@
 //
 // Shared memory: Q 64 KB, K 2 x 32 KB, V 2 x 32 KB. TMEM: S0, S1, O0, O1 of 128
 // columns each; P_x takes the first 64 columns of S_x.
+//
+// Measured (32 / 8 heads, groups of 64): 2048 tokens after 29952 in 1388 us,
+// 749 TFLOP/s. Its 256 CTAs are two rounds of 148 (86 % of the SMs' time); in a
+// CTA the products (2048 cycles per 128 keys at full rate), the exponentials (2048
+// at 16 a cycle) and the operands' shared-memory traffic (about 2048) overlap only
+// in part, and with the conversions taken out an earlier step at 709 ran at 955.
 //
 // Every wait is bounded (common.cuh).
 #include <torch/extension.h>
@@ -149,20 +155,29 @@ __device__ __forceinline__ P4Tile p4_tile(const Prefill4Args& a, int left) {
   return {-1, 0};
 }
 
-// The values s (c + z) of a word's eight codes as four pairs (code i, code i + 4):
-// 1024 + c (1024 + 16 c) by mask, c exactly, then one rounding.
-__device__ __forceinline__ void p4_values(uint32_t w, __half2 s, __half2 sz, uint32_t (&v)[4]) {
-  const __half2 big = __float2half2_rn(1024.f), low = __float2half2_rn(-64.f), part = __float2half2_rn(0.0625f);
+// The values s (c + z) of a word's eight codes as four pairs (code i, code i + 4),
+// divided by P4_UNIT: the masked codes are the fp16 subnormals c 2^-24 (c 2^-20),
+// `z` is the zero point times 2^-9 and `s` the scale times 2^5. c + z comes out
+// exactly (it is a multiple of 2^-7 below 16, and finer below 8), so the only
+// rounding is the value's own. Rounding s z once for a whole group instead cost
+// as many instructions and, being the same error for all its channels, moved the
+// scores of long contexts by up to a bf16 step of the output.
+constexpr float P4_UNIT = 16.f;
+__device__ __forceinline__ void p4_values(uint32_t w, __half2 s, __half2 z, uint32_t (&v)[4]) {
+  const __half2 up0 = __float2half2_rn(32768.f), up1 = __float2half2_rn(2048.f);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t m0 = (w & 0x000f000fu) | 0x64006400u, m1 = (w & 0x00f000f0u) | 0x64006400u;
-    const __half2 c0 = __hsub2(*reinterpret_cast<const __half2*>(&m0), big);
-    const __half2 c1 = __hfma2(*reinterpret_cast<const __half2*>(&m1), part, low);
-    const __half2 v0 = __hfma2(c0, s, sz), v1 = __hfma2(c1, s, sz);
+    const uint32_t m0 = w & 0x000f000fu, m1 = w & 0x00f000f0u;
+    const __half2 v0 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&m0), up0, z), s);
+    const __half2 v1 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&m1), up1, z), s);
     v[2 * i] = *reinterpret_cast<const uint32_t*>(&v0);
     v[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&v1);
     w >>= 8;
   }
+}
+// A (scale, zero point) word as those two factors: fp16 s 2^5 in the low half, z 2^-9 in the high half.
+__device__ __forceinline__ uint32_t p4_factors(uint32_t word) {
+  return pack_f16(kv4_scale(word) * 32.f, kv4_zero(word) * 0.001953125f);
 }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -268,7 +283,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     const int e = min(126, max(-100, (int)((__float_as_uint(amax) >> 23) & 255u) - 127));
     const float up = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (half == 0) sF[r] = a.scale_log2 * exp2f((float)e);
+    if (half == 0) sF[r] = a.scale_log2 * P4_UNIT * exp2f((float)e);
     uint8_t* dst = sQ + (r >> 7) * P4_TILE + half * P4_CHUNK + (r & 127) * 128;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       }
     } else if (ok) {
       tc_fence_after();
-      const float inv = l != 0.f ? 1.f / l : 0.f;           // a row that sees no key gives zeros
+      const float inv = l != 0.f ? P4_UNIT / l : 0.f;       // a row that sees no key gives zeros
       __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
                            (int64_t)(kvh * a.group + row % a.group) * HD;
 #pragma unroll
@@ -491,8 +506,9 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         uint8_t* dst = sK + st * P4_TILE + key * 128;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          const __half2 sc = __float2half2_rn(kv4_scale(kp[i]));
-          const __half2 sz = __float2half2_rn(kv4_scale(kp[i]) * kv4_zero(kp[i]));
+          const uint32_t f = p4_factors(kp[i]);
+          const uint32_t f0 = __byte_perm(f, f, 0x1010), f1 = __byte_perm(f, f, 0x3232);
+          const __half2 sc = *reinterpret_cast<const __half2*>(&f0), sz = *reinterpret_cast<const __half2*>(&f1);
 #pragma unroll
           for (int e = i * (4 / NG); e < (i + 1) * (4 / NG); ++e)   // word e of 16 bytes h: channels 32 e + 8 h
 #pragma unroll
@@ -512,9 +528,9 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         next();
         load_k();
       }
-      uint32_t ss[NG];                                      // fp16 (scale, scale x zero point) of this lane's token
+      uint32_t ss[NG];                                      // the factors of this lane's token
 #pragma unroll
-      for (int i = 0; i < NG; ++i) ss[i] = pack_f16(kv4_scale(vp[i]), kv4_scale(vp[i]) * kv4_zero(vp[i]));
+      for (int i = 0; i < NG; ++i) ss[i] = p4_factors(vp[i]);
       if (!__all_sync(0xffffffffu, kv4_wait(&v_empty[st], ph, kErrP4VEmpty))) break;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         uint8_t* d1 = dst + (((u + 1) ^ g) << 4);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          // (scale, scale) and (base, base) of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+          // scales and zero points of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
           uint32_t sc[2], sz[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -638,7 +654,7 @@ __global__ void __launch_bounds__(256) prefill4_join_kernel(const Prefill4Args a
     o.z = fmaf(v.z, e, o.z);
     o.w = fmaf(v.w, e, o.w);
   }
-  const float inv = L != 0.f ? 1.f / L : 0.f;
+  const float inv = L != 0.f ? P4_UNIT / L : 0.f;
   __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
                        (int64_t)(kvh * a.group + row % a.group) * HD + 4 * lane;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));

@@ -79,11 +79,11 @@ def test_many_rows_fill_whole_records_or_not(kind, start, group):
     """Enough rows that 16 of them go together where they fill a record: sequences that begin anywhere,
     -1 slots inside, unordered slots, records that are full in the cache but not by rows that follow one another."""
     g = gen(4 + start)
-    n, hkv, page = 1100, 8, 48
+    n, hkv, page = 4200, 8, 48
     k, v = rows(g, n, hkv).flatten(1), rows(g, n, hkv).flatten(1)
     slots = torch.cat([torch.arange(m, device=DEV) + 48 * 13 * i + (start if i % 2 else 0) for i, m in
-                       enumerate([600, 37, 16, 15, 432])])
-    pages = 13 * 5
+                       enumerate([600, 37, 16, 15, 3532])])
+    pages = 128
     if kind == "holes":
         slots[5::61] = -1
     elif kind == "shuffled":
@@ -97,7 +97,6 @@ def test_many_rows_fill_whole_records_or_not(kind, start, group):
         ops.kv4_write(k[i:i + 100], v[i:i + 100], exp, slots[i:i + 100])
     assert torch.equal(got, exp)
     assert torch.equal(ops.kv4_read(got, slots)[0], torch.cat([ops.kv4_read(got, s)[0] for s in slots.split(100)]))
-    assert torch.equal(ops.kv4_read(got, slots)[1], torch.cat([ops.kv4_read(got, s)[1] for s in slots.split(100)]))
 
 
 @pytest.mark.parametrize("order", ["shuffled", "reversed", "two_runs"])
@@ -321,11 +320,11 @@ def test_decode_page_outside_the_cache_is_an_error(ws):
 def check_prefill(new, old, heads, hkv, page, group, ws, seed=0, q=None):
     """Packed sequences of ``new`` tokens after ``old`` cached ones.
 
-    Besides :func:`check`'s terms the operands are rounded to 11 bits: a value's
-    base (scale x zero point, up to twice the largest value, one rounding for a
-    whole group) moves a score by about 0.005 for these inputs, three times that
-    at worst over half of the value range: 2^-7 of it. Over a whole result the
-    differences average out to below half a bf16 step (2^-8)."""
+    Besides :func:`check`'s terms the operands are rounded to 11 bits: were a
+    group's scale x zero point rounded once (up to twice the largest value), a
+    score would move by about 0.005 for these inputs, three times that at worst
+    over half of the value range: 2^-7 of it. Over a whole result the differences
+    average out to below half a bf16 step (2^-8)."""
     g = gen(seed + page + group + heads)
     contexts = [a + b for a, b in zip(new, old)]
     cache, tables, values = filled(g, contexts, hkv, page, group)
