@@ -11,7 +11,8 @@ With ``kv_group`` the cache holds 4-bit codes instead: one uint8 tensor per laye
 
 A request can be forked (full pages shared by reference, the partly filled one
 copied) and the pool compacted (live pages moved to its front); both move pages of
-every layer with one kernel.
+every layer with one kernel on the current stream, which has to be the one that the
+forwards use (or ordered with it on both sides).
 
 Pages are sized from the HBM left after weights, LoRA buffers and the
 activation-capture buffers (``gpu_memory_utilization`` of the total).

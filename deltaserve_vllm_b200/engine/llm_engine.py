@@ -631,7 +631,8 @@ class CoServingEngine:
                         block_hashes=list(r.block_hashes))
         child.output_logprobs = list(r.output_logprobs)
         child.output_top_logprobs = list(r.output_top_logprobs)
-        child.block_ids = self.kv.fork([(r.block_ids, r.num_computed)])[0]
+        with torch.cuda.stream(self.fwd_stream):  # behind the last forward, ahead of the next
+            child.block_ids = self.kv.fork([(r.block_ids, r.num_computed)])[0]
         child.num_registered = min(r.num_registered, r.num_computed // self.kv.block_size)
         self.scheduler.running.append(child)
         self.requests[new_id] = child
@@ -645,7 +646,8 @@ class CoServingEngine:
         if self.tp_size > 1:
             raise ValueError("compact_kv needs tensor_parallel_size 1")
         held = list(self.scheduler.running) + list(self.scheduler.waiting)
-        return self.kv.compact([r.block_ids for r in held])
+        with torch.cuda.stream(self.fwd_stream):  # behind the last forward, ahead of the next
+            return self.kv.compact([r.block_ids for r in held])
 
     def abort_request(self, request_id: str) -> bool:
         if self.router is not None and self.router.cancel(request_id):

@@ -178,3 +178,31 @@ def test_comparison_command_runs():
                 "--blocks", "16"])
     assert res["int4"]["page_bytes"] * 2 * 256 == res["auto"]["page_bytes"] * 72      # fp32 pages on CPU
     assert res["int4"]["fork"]["same_tokens"]
+
+
+def test_fork_and_compact_copy_on_the_forward_stream(monkeypatch):
+    """The pages that move are the forward's: their copies belong to the stream it runs on, whatever the caller's is."""
+    eng = engine()
+    for i, p in enumerate(prompts(3)):
+        eng.add_request(f"r{i}", p, SamplingParams(max_tokens=8))
+    while len(eng.requests["r2"].output_ids) < 3:
+        eng.step()
+    current, copied = ["caller's"], []
+
+    class On:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            current.append(self.stream)
+
+        def __exit__(self, *exc):
+            current.pop()
+    copy = ops.copy_pages
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    monkeypatch.setattr(ops, "copy_pages", lambda *a: (copied.append((current[-1], len(a[1]))), copy(*a)))
+    monkeypatch.setattr(eng, "fwd_stream", "forward")
+    eng.fork_request("r2", "fork")
+    eng.scheduler.abort("r1")                     # leaves holes for the compaction
+    eng.compact_kv()
+    assert [s for s, _ in copied] == ["forward"] * 2 and all(n for _, n in copied)

@@ -110,3 +110,63 @@ def test_fork_and_compact(dtype):
     got = {r.request_id: r.output_ids for r in eng.finished}
     assert got["fork"] == got["r2"] and len(got["r1"]) == 20
     assert eng.kv.allocator.num_free == eng.kv.allocator.num_blocks
+
+
+def _busy(stream, n=60):
+    """Plain work that keeps ``stream`` busy for some 50 ms."""
+    with torch.cuda.stream(stream):
+        a = torch.ones(8192, 8192, device="cuda", dtype=torch.bfloat16)
+        for _ in range(n):
+            a @ a
+
+
+def _serve(dtype, lengths, budget=2048, **tokens):
+    ecfg = EngineConfig(model="llama3-test", max_model_len=1024, block_size=64, max_num_batched_tokens=budget, max_loras=2,
+                        max_lora_rank=16, num_gpu_blocks_override=64, kv_cache_dtype=dtype)
+    eng = CoServingEngine(ecfg, FinetuneConfig(enable_finetuning=False))
+    g = torch.Generator().manual_seed(3)
+    for i, n in enumerate(lengths):
+        eng.add_request(f"r{i}", torch.randint(0, 4096, (n,), generator=g).tolist(),
+                        SamplingParams(max_tokens=tokens.get(f"r{i}", 16)))
+    return eng
+
+
+@pytest.mark.parametrize("dtype", ["int4", "auto"])
+def test_fork_and_compact_with_a_busy_caller(dtype):
+    """The caller's stream is far behind: the next forward still finds the pages copied, and no copy comes after it."""
+    eng = _serve(dtype, (100, 300, 90), r0=2)
+    while len(eng.requests["r2"].output_ids) < 4:
+        eng.step()
+    _busy(torch.cuda.current_stream())
+    eng.fork_request("r2", "fork")
+    eng.step()
+    _busy(torch.cuda.current_stream())
+    eng.compact_kv()
+    eng.run_until_idle(max_steps=500)
+    torch.cuda.synchronize()
+    assert ops.check_device_error() == 0
+    plain = _serve(dtype, (100, 300, 90), r0=2)
+    plain.run_until_idle(max_steps=500)
+    got = {r.request_id: r.output_ids for r in eng.finished}
+    exp = {r.request_id: r.output_ids for r in plain.finished}
+    assert got["fork"] == got["r2"] and got["r2"][:4] == exp["r2"][:4]
+
+
+@pytest.mark.parametrize("dtype", ["int4", "auto"])
+def test_compact_behind_a_running_chunk(dtype):
+    """A prefill chunk that samples nothing is still running when its pages are moved."""
+    def run(compact):
+        eng = _serve(dtype, (300, 900), budget=128, r0=2)
+        while any(r.request_id == "r0" for r in eng.scheduler.running + list(eng.scheduler.waiting)):
+            eng.step()
+        r1 = eng.requests["r1"]
+        before, at = list(r1.block_ids), r1.num_computed
+        _busy(eng.fwd_stream)
+        eng.step()
+        assert r1.in_prefill and r1.num_computed > at
+        if compact:
+            eng.compact_kv()
+            assert r1.block_ids[:len(before)] != before
+        eng.run_until_idle(max_steps=500)
+        return r1.output_ids
+    assert run(True) == run(False)
