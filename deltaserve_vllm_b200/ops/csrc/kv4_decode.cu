@@ -252,10 +252,11 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
         const int g0 = max(lo, x & ~7), g1 = min(hi, x | 7);        // our group of eight
         auto left = [&](int y) { return max(f, y << (3 * level)); };   // a node's data lies with its leftmost run
         if (g1 > g0) {
-          __syncwarp();                      // lane 0 releases every lane's part and acquires the others'
+          __syncwarp();                      // lane 0 releases every lane's part
           int old = 0;
           int* count = a.arrived + level * 2 * runs + slot(left(g0));
           if (lane == 0) old = atom_add_acq_rel(count, 1);
+          __syncwarp();                      // and acquires the others' for every lane
           old = __shfl_sync(0xffffffffu, old, 0);
           if (old != g1 - g0) break;
           if (lane == 0) *count = 0;
