@@ -11,6 +11,7 @@ silent fallback.
 from __future__ import annotations
 
 import os
+import weakref
 
 import torch
 
@@ -47,11 +48,22 @@ def _native(kernels: int = 1):
     return _EXT
 
 
+# Workspaces that hold state between calls (arrival counters, zero at rest).
+_STATEFUL: list[weakref.ref] = []
+
+
 def check_device_error(clear: bool = True) -> int:
-    """Error code written by a kernel whose bounded wait gave up (0 = none)."""
+    """Error code written by a kernel whose bounded wait gave up (0 = none).
+    Clearing one also returns the workspaces to their initial state."""
     if _EXT is None or not torch.cuda.is_available():
         return 0
-    return int(_EXT.read_error(clear))
+    code = int(_EXT.read_error(clear))
+    if code and clear:
+        for ws in [ws for r in _STATEFUL if (ws := r()) is not None]:
+            torch.cuda.synchronize(ws.device)
+            ws.zero_()
+            torch.cuda.synchronize(ws.device)
+    return code
 
 
 # ----------------------------------------------------------------- GEMM
@@ -278,7 +290,10 @@ def kv4_workspace(device):
     one each)."""
     device = torch.device(device)
     n = _native(0).kv4_workspace_bytes() if device.type == "cuda" else 0
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    ws = torch.zeros(n, dtype=torch.uint8, device=device)
+    if n:
+        _STATEFUL[:] = [r for r in _STATEFUL if r() is not None] + [weakref.ref(ws)]
+    return ws
 
 
 def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws):

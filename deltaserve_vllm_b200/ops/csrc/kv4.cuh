@@ -318,6 +318,12 @@ struct Kv4Warp {
     }
   }
 
+  // The result becomes NaN.
+  __device__ __forceinline__ void poison() {
+#pragma unroll
+    for (int n = 0; n < NH; ++n) l[n][0] = l[n][1] = __uint_as_float(0x7fffffffu);
+  }
+
   // Sum the lanes' shares and complete the output: afterwards acc[n][i][e] is
   // the unnormalised output of channel 16 i + g + 8 (e / 2), column
   // 8 n + 2 t + e % 2.

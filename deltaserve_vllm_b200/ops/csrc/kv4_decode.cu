@@ -212,12 +212,14 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
   Warp acc;
   int st = 0;
   uint32_t phase = 0;
+  bool ok = true;                             // no wait has given up
   for (int at = first; at < last;) {
     const int c0 = w.c, c1 = min(w.n, c0 + (last - at));
     const __nv_bfloat16* q = a.q + w.b * a.q_stride + (int64_t)w.h * a.group * HD;
     acc.begin([&](int col) { return col < a.group ? q + col * HD : (const __nv_bfloat16*)nullptr; }, a.scale_log2);
-    for (int c = c0; c < c1; ++c) {
-      if (!__all_sync(0xffffffffu, kv4_wait(&full[st], phase, kErrD4Full))) {
+    for (int c = c0; c < c1 && ok; ++c) {
+      ok = __all_sync(0xffffffffu, kv4_wait(&full[st], phase, kErrD4Full));
+      if (!ok) {
         // The copies under way land before the CTA gives its memory back.
         for (int left = issued - at - (c - c0); left > 0; --left) {
           kv4_drain(&full[st], phase);
@@ -226,8 +228,7 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
             phase ^= 1u;
           }
         }
-        cp_async_wait<0>();
-        return;
+        break;
       }
       acc.tokens(ring + st * (2 * REC), w.len - c * 32);
       __syncwarp();
@@ -237,6 +238,9 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
         phase ^= 1u;
       }
     }
+    // After a wait that gave up every segment of the run still arrives at its
+    // joins, as NaN: the counters return to zero and no later call waits for it.
+    if (!ok) acc.poison();
     acc.finish();
     __nv_bfloat16* out = a.out + w.b * a.out_stride + (int64_t)w.h * a.group * HD;
     bool done = c0 == 0 && c1 == w.n;

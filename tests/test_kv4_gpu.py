@@ -317,6 +317,20 @@ def test_decode_page_outside_the_cache_is_an_error(ws):
     assert ops.check_device_error() != 0
 
 
+def test_an_error_leaves_no_state_behind(ws):
+    """Clearing an error returns a workspace's arrival counters to zero, whatever the failed call left in them."""
+    g = gen(15)
+    cache, tables, _ = filled(g, [3000, 90], 2, 64, 64)
+    ctx = torch.tensor([3000, 90], dtype=torch.int32, device=DEV)
+    q = torch.randn(2, 8 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    exp = ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, ws)
+    used = ops.kv4_workspace(DEV)
+    used.fill_(1)
+    ops.kv4_write(rows(g, 1, 2), rows(g, 1, 2), cache, torch.tensor([1 << 40], device=DEV))
+    assert ops.check_device_error() != 0
+    assert torch.equal(ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, used), exp)
+
+
 def check_prefill(new, old, heads, hkv, page, group, ws, seed=0, q=None):
     """Packed sequences of ``new`` tokens after ``old`` cached ones.
 
