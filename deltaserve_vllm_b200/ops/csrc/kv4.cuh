@@ -11,8 +11,8 @@
 //
 // over the group's inputs, which saturate at +-8192 (a NaN counts as 0); a
 // group whose step is below 2^-120 is stored as zeros. The limit keeps s below
-// 2^10.1, so that s * p (p a softmax weight below 2^5) and s * (c + z) fit fp16;
-// the scale itself is bf16 so that small groups keep their relative precision.
+// 2^10.1; the scale is bf16 so that small groups keep their relative precision
+// (the kernels take a power of two out of it before anything becomes fp16).
 //
 // Order of the codes. The matrix instruction m16n8k16 takes its A operand as
 // 16-bit pairs; a 32-bit word of 8 codes gives four pairs by masking, because
@@ -101,11 +101,20 @@ __device__ __forceinline__ void kv4_drain(uint64_t* bar, uint32_t parity) {
 // instruction as fp16 subnormals and the query as fp16 scaled by a power of two
 // per column (its largest magnitude lands in [2^14, 2^15); bf16 fits fp16's
 // mantissa, so this is exact down to 2^-29 of the largest), and the products
-// are undone by `f`. Output: O = sum p s c + sum p s z: p s is rounded to fp16
-// (11 bits) for the matrix instruction, the second sum is one fp32 number per
-// group and column.
+// are undone by `f`. Output: O = sum w c + sum w z with w = p s 2^-r rounded to
+// fp16 (11 bits), the second sum one fp32 number per group and column. Both sums
+// take the rounded w, so that a weight's rounding scales its key's value as a
+// whole. Each group of channels has its own power of two, r: it puts the group's
+// largest scale into [2^7, 2^8) and moves, as the reference maximum does, when one
+// of 2^10 or more comes. So w stays below 2^15, and a key keeps its 11 bits down
+// to 2^-23 of the largest p s of its group, whatever the values' size (a fixed r
+// lost small groups altogether, and the small weights beside a dominant key: 4 %
+// of the result for values near 1e-6).
 constexpr float KV4_P_BIAS = 2.f;
 constexpr float KV4_LAZY = 3.f;
+constexpr int KV4_R_TOP = 7;
+constexpr uint32_t KV4_R_SUM = (127u + KV4_R_TOP + 127 + 3) << 23;   // bits of 2^-r plus those of the scale that moves it
+constexpr int KV4_R_MIN = -110;              // exponent of the smallest scale that r follows: 2^-r stays finite
 
 template <int NG, int NH>
 struct Kv4Warp {
@@ -113,7 +122,8 @@ struct Kv4Warp {
   float f[NH][2];         // score factor of columns 2t, 2t + 1
   float qs[NH][NG][2];    // scaled sum of the query over each group
   float acc[NH][8][4];    // sum p s c, channels 16 m + g (+ 8: times 16) x columns 2t, 2t + 1; times 2^-24
-  float z[NH][NG][2];     // this lane's share of sum p s z
+  float z[NH][NG][2];     // this lane's share of sum w z
+  float* rs;              // 2^-r of each group, in shared memory: registers are short
   float m[NH][2], l[NH][2];
   float ref[NH][2];       // what scores are taken against: m - KV4_P_BIAS, 0 before the first
 
@@ -184,6 +194,11 @@ struct Kv4Warp {
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
     }
+    __syncwarp();                            // the last segment's readers are done
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      if (lane == 0) rs[i] = __uint_as_float((uint32_t)(127 + KV4_R_TOP - KV4_R_MIN) << 23);
+    __syncwarp();
   }
 
   // Two K and V records (32 tokens; 16-byte aligned), of which the first `valid`
@@ -246,6 +261,15 @@ struct Kv4Warp {
     }
     float top[NH][2];
     bool grow = false;
+    // The V scales, one token per lane. As bits they are ordered, and the zero
+    // point below one does not change which power of two it reaches.
+    const uint8_t* scales = rec + (lane >> 4) * 2 * KREC + KREC + KV4_CODES + 4 * (lane & 15);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      uint32_t x = *reinterpret_cast<const uint32_t*>(scales + 64 * i);
+      if (!ALL && lane >= valid) x = 0;
+      grow |= x >= KV4_R_SUM - __float_as_uint(rs[i]);
+    }
 #pragma unroll
     for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -254,6 +278,19 @@ struct Kv4Warp {
         grow |= top[n][c] > m[n][c] + KV4_LAZY;
       }
     if (__any_sync(0xffffffffu, grow)) {
+      float move[NG];                        // of each group's sums
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        uint32_t x = *reinterpret_cast<const uint32_t*>(scales + 64 * i);
+        if (!ALL && lane >= valid) x = 0;
+        // a scale is below 2^11: what is not one (a NaN) moves r no further
+        const int e = min(11, (int)(__reduce_max_sync(0xffffffffu, x) >> 23 & 255u) - 127);
+        const float from = rs[i], to = fminf(from, __uint_as_float((uint32_t)(127 + KV4_R_TOP - max(e, KV4_R_MIN)) << 23));
+        move[i] = __uint_as_float(__float_as_uint(to) - __float_as_uint(from) + (127u << 23));
+        __syncwarp();
+        if (lane == 0) rs[i] = to;
+      }
+      __syncwarp();
 #pragma unroll
       for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -267,11 +304,11 @@ struct Kv4Warp {
           ref[n][c] = mx == -INFINITY ? 0.f : mx - KV4_P_BIAS;
           l[n][c] *= corr;
 #pragma unroll
-          for (int i = 0; i < NG; ++i) z[n][i][c] *= corr;
+          for (int i = 0; i < NG; ++i) z[n][i][c] *= corr * move[i];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            acc[n][i][c] *= corr;
-            acc[n][i][2 + c] *= corr;
+            acc[n][i][c] *= corr * move[i * NG / 8];
+            acc[n][i][2 + c] *= corr * move[i * NG / 8];
           }
         }
     }
@@ -295,16 +332,17 @@ struct Kv4Warp {
         uint32_t p0 = vp[ng * 16], p1 = vp[ng * 16 + 8];
         if (!ALL && 16 * r + g >= valid) p0 = 0;
         if (!ALL && 16 * r + g + 8 >= valid) p1 = 0;
-        const float s0 = kv4_scale(p0), s1 = kv4_scale(p1);
-        const float b0 = s0 * kv4_zero(p0), b1 = s1 * kv4_zero(p1);
+        const float s0 = kv4_scale(p0) * rs[ng], s1 = kv4_scale(p1) * rs[ng];
+        const float z0 = kv4_zero(p0), z1 = kv4_zero(p1);
         uint32_t w[NH][2];
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
           const float* p = &s[n][4 * r];
-          w[n][0] = movm_t(pack_f16(p[0] * s0, p[1] * s0));
-          w[n][1] = movm_t(pack_f16(p[2] * s1, p[3] * s1));
-#pragma unroll
-          for (int c = 0; c < 2; ++c) z[n][ng][c] = fmaf(p[c], b0, fmaf(p[2 + c], b1, z[n][ng][c]));
+          const __half2 h0 = __floats2half2_rn(p[0] * s0, p[1] * s0), h1 = __floats2half2_rn(p[2] * s1, p[3] * s1);
+          w[n][0] = movm_t(*reinterpret_cast<const uint32_t*>(&h0));
+          w[n][1] = movm_t(*reinterpret_cast<const uint32_t*>(&h1));
+          z[n][ng][0] = fmaf(__low2float(h0), z0, fmaf(__low2float(h1), z1, z[n][ng][0]));
+          z[n][ng][1] = fmaf(__high2float(h0), z0, fmaf(__high2float(h1), z1, z[n][ng][1]));
         }
 #pragma unroll
         for (int j = 0; j < 8 / NG; ++j) {
@@ -328,6 +366,9 @@ struct Kv4Warp {
   // the unnormalised output of channel 16 i + g + 8 (e / 2), column
   // 8 n + 2 t + e % 2.
   __device__ __forceinline__ void finish() {
+    float r[NG];                             // 2^r
+#pragma unroll
+    for (int i = 0; i < NG; ++i) r[i] = __uint_as_float((254u << 23) - __float_as_uint(rs[i]));
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
 #pragma unroll
@@ -342,7 +383,7 @@ struct Kv4Warp {
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          acc[n][i][e] = fmaf(acc[n][i][e], e < 2 ? 16777216.f : 1048576.f, z[n][i * NG / 8][e & 1]);
+          acc[n][i][e] = fmaf(acc[n][i][e], e < 2 ? 16777216.f : 1048576.f, z[n][i * NG / 8][e & 1]) * r[i * NG / 8];
     }
   }
 

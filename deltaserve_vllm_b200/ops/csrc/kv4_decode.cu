@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
   using Warp = Kv4Warp<NG, NH>;
   __shared__ uint64_t full_bars[D4_WARPS][D4_MAX_STAGES];
   __shared__ int page_ids[D4_WARPS][D4_PAGES];
+  __shared__ float rs[D4_WARPS][NG];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   uint8_t* ring = d4_smem + warp * a.stages * (2 * REC);
   uint64_t* full = full_bars[warp];
@@ -210,6 +211,7 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
   for (int i = 0; i < a.stages && issued < last; ++i) fetch();
 
   Warp acc;
+  acc.rs = rs[warp];
   int st = 0;
   uint32_t phase = 0;
   bool ok = true;                             // no wait has given up
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
 template <int NG, int NH, int MIN_CTAS>
 static void decode4_launch(Decode4Args a, int sms, cudaStream_t stream) {
   constexpr int STAGE = 4 * kv4_record(NG);
-  constexpr int ROOM = 227 * 1024 / MIN_CTAS - 1024 - D4_WARPS * (D4_MAX_STAGES * 8 + D4_PAGES * 4);
+  constexpr int ROOM = 227 * 1024 / MIN_CTAS - 1024 - D4_WARPS * (D4_MAX_STAGES * 8 + D4_PAGES * 4 + NG * 4);
   a.stages = std::min(D4_MAX_STAGES, ROOM / (D4_WARPS * STAGE));
   const int smem = D4_WARPS * a.stages * STAGE;
   static const cudaError_t attr =

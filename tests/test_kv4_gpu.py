@@ -461,6 +461,128 @@ def test_prefill_page_outside_the_cache_is_an_error(ws):
     assert ops.check_device_error() != 0
 
 
+# ----------------------------------------------------------------- magnitudes
+
+def held(g, k, v, page, group):
+    """One sequence's cache of the rows k / v [n, hkv, 128], its table and the values it stands for: float64 [hkv, n, 128] each."""
+    n, hkv = k.shape[:2]
+    need = -(-n // page)
+    perm = torch.randperm(need + 1, generator=g, device=DEV)[:need]
+    cache = empty_cache(need + 1, hkv, page, group)
+    pos = torch.arange(n, device=DEV)
+    ops.kv4_write(k.to(torch.bfloat16), v.to(torch.bfloat16), cache, perm[pos // page] * page + pos % page)
+    rec = ref.kv4_values(cache[perm]).double()
+    return cache, perm.to(torch.int32)[None], [rec[:, :, :, w].permute(1, 0, 2, 3, 4).reshape(hkv, -1, 128)[:, :n]
+                                               for w in (0, 1)]
+
+
+def attend(op, q, cache, tables, n, ws):
+    """The last len(q) queries of n cached tokens, by prefill, or each over all of them, by decode."""
+    m, heads = q.shape[0], q.shape[1] // 128
+    out = torch.full_like(q, float("nan"))
+    if op == "decode":
+        ctx = torch.full((m,), n, dtype=torch.int32, device=DEV)
+        return ops.paged_decode4(q, cache, tables.expand(m, -1).contiguous(), ctx, out, heads, SCALE, ws)
+    cu = torch.tensor([0, m], dtype=torch.int32, device=DEV)
+    return ops.paged_prefill4(q, cache, tables, cu, torch.tensor([n], dtype=torch.int32, device=DEV), out, heads, SCALE, ws)
+
+
+def check_magnitudes(op, q, k, v, page, group, ws, g):
+    """Every row's every channel group against its own norm.
+
+    The result is rounded to bf16 (2^-9 of each channel) and its weights have a common error (of the sum, of a dominant
+    key's score) of up to 2^-9: together 2^-8 of the norm. Each key's share p |v| is off by its own roundings to 11 bits
+    (weight; in prefill K's and V's two each, those of K moving a score of a few units by some 2^-11): independent
+    between keys, rms below 2^-10 sqrt(sum (p |v|)^2), of which twice is allowed."""
+    n, hkv = k.shape[:2]
+    cache, tables, (k64, v64) = held(g, k, v, page, group)
+    got = attend(op, q, cache, tables, n, ws).double().view(q.shape[0], hkv, -1, 128 // group, group)
+    qq = q.double().view(q.shape[0], hkv, -1, 128)
+    s = torch.einsum("mhgd,hkd->mhgk", qq, k64) * SCALE
+    if op == "prefill":
+        late = torch.arange(n, device=DEV)[None] > n - q.shape[0] + torch.arange(q.shape[0], device=DEV)[:, None]
+        s = s.masked_fill(late[:, None, None], float("-inf"))
+    p = torch.softmax(s, -1)
+    exp = torch.einsum("mhgk,hkd->mhgd", p, v64).unflatten(-1, (-1, group))
+    share = torch.einsum("mhgk,hkx->mhgx", p * p, v64.unflatten(-1, (-1, group)).square().sum(-1)).sqrt()
+    err, bound = (got - exp).norm(dim=-1), 2 ** -8 * exp.norm(dim=-1) + 2 ** -9 * share
+    assert bool((err <= bound).all()), float((err / bound).max())
+    return p
+
+
+OPS = ["decode"]
+
+
+@pytest.mark.parametrize("group", ops.KV4_GROUPS)
+@pytest.mark.parametrize("size", [1e3, 1.0, 1e-2, 1e-4, 1e-5, 1e-6, 1e-7, 1e-12, 1e-30])
+@pytest.mark.parametrize("op", OPS)
+def test_values_of_any_size(op, size, group, ws):
+    g = gen(30)
+    q = torch.randn(5, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    check_magnitudes(op, q, rows(g, 700, 2).float(), rows(g, 700, 2).float() * size, 64, group, ws, g)
+
+
+@pytest.mark.parametrize("size", [1e4, 1.0, 1e-3, 1e-5, 1e-6, 1e-9, 1e-20])
+@pytest.mark.parametrize("op", OPS)
+def test_keys_of_any_size(op, size, ws):
+    """Keys that are small where queries are large: the scores are the same."""
+    g = gen(31)
+    q = (torch.randn(5, 4 * 128, generator=g, device=DEV) / size * 1.5).to(torch.bfloat16)
+    k = torch.randn(700, 2, 128, generator=g, device=DEV) * size
+    check_magnitudes(op, q, k.clamp(-8000, 8000), rows(g, 700, 2).float(), 64, 64, ws, g)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_tokens_of_different_sizes(op, ws):
+    """Values from 1e-6 to 1e2 side by side, small ones first and last."""
+    g = gen(32)
+    n = 1500
+    size = 10 ** (torch.rand(n, generator=g, device=DEV) * 8 - 6)
+    size[:200] = 1e-6
+    size[-300:] = 1e-4
+    q = torch.randn(5, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    check_magnitudes(op, q, rows(g, n, 2, wide=1.0).float(), rows(g, n, 2).float() * size[:, None, None], 48, 32, ws, g)
+
+
+@pytest.mark.parametrize("op", OPS)
+def test_zero_values_before_others(op, ws):
+    """Pieces whose groups are all zero, and then values of an ordinary size."""
+    g = gen(33)
+    v = rows(g, 900, 2).float()
+    v[:400] = 0
+    v[-130:] = 0
+    q = torch.randn(5, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    check_magnitudes(op, q, rows(g, 900, 2, wide=1.0).float(), v, 64, 64, ws, g)
+
+
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("op", OPS)
+def test_channel_groups_of_different_sizes(op, group, ws):
+    """A group of channels 1e6 times smaller than its neighbours is as precise as they are."""
+    g = gen(34)
+    v = rows(g, 3000, 1).float()
+    v[..., group:2 * group] *= 1e-6
+    q = torch.randn(3, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    check_magnitudes(op, q, rows(g, 3000, 1, wide=1.0).float(), v, 64, group, ws, g)
+
+
+@pytest.mark.parametrize("at", [0, 17000, -40])
+@pytest.mark.parametrize("nats,size", [(10.0, 1.0), (13.0, 1.0), (13.0, 1e-2), (14.0, 1e-5), (15.5, 1e-2)])
+@pytest.mark.parametrize("op", OPS)
+def test_a_dominant_key_with_a_small_value_row(op, nats, size, at, ws):
+    """One key of 32768 takes most of the weight and has next to no value: the others' small weights make the result."""
+    g = gen(35)
+    n = 32768
+    u = torch.randn(128, generator=g, device=DEV).sign()
+    q = (u + 0.2 * torch.randn(3, 4, 128, generator=g, device=DEV)).flatten(1).to(torch.bfloat16)
+    k = torch.randn(n, 1, 128, generator=g, device=DEV) * 0.5
+    k[at] = u * nats / (128 * SCALE)
+    v = torch.randn(n, 1, 128, generator=g, device=DEV) * size
+    v[at] *= 1e-5
+    p = check_magnitudes(op, q, k, v, 64, 64, ws, g)
+    assert float(p.amax(-1).min()) > 0.3
+
+
 @pytest.mark.parametrize("kind", ["int4", "bf16", "bytes16"])
 @pytest.mark.parametrize("layers,pages,moves", [(1, 2, 1), (3, 40, 20), (200, 9, 3), (2, 1300, 600)])
 def test_copy_pages(kind, layers, pages, moves):
