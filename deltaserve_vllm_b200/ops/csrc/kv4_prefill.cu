@@ -19,11 +19,17 @@
 //   warp 12          issues the MMAs: S_x = Q_x K^T, then O_x += P_x V with P
 //                    from TMEM. Tile 0's softmax runs while tile 1's products do.
 //
-// Operands are fp16 (fp32 accumulators): a value s (c + z) of the 4-bit format
-// fits its 11 bits to within 2^-12 of itself, where bf16 operands would double the
-// result's own rounding error. K and V enter divided by 16 (below 545) and P below
-// 2^8; each query row is scaled by a power of two (its largest magnitude lands
-// in [1, 2)), which the softmax undoes.
+// Operands are fp16 (fp32 accumulators): a value s (c + z) of the 4-bit format is
+// off by at most 2^-10 of itself (two roundings to 11 bits, see p4_values), where
+// bf16 operands would double the result's own rounding error. fp16 has few
+// exponents, so every operand enters relative to a power of two of its own: K to
+// that of the largest scale of a warp's 32 keys (undone on the score), V to that of
+// the largest scale so far of each group of channels (a larger one rescales O, as a
+// larger maximum does), each query row to that of its largest magnitude, and P to a
+// reference that puts the largest weight between 2^11 and 2^15. A value keeps its
+// bits down to 2^-24 of the largest, a weight to 2^-25. (With fixed divisors of 16
+// values near 1e-5 were off by 3 %, and weights of 2^-16 beside a dominant key by
+// their rounding to subnormals.)
 //
 // K is stored as [keys x channels], V as [channels x keys] (both K-major for
 // their product): the code pairs that one mask yields, channels (c, c + 4) of
@@ -56,8 +62,9 @@ namespace dsv {
 constexpr int P4_THREADS = 512;
 constexpr int P4_CHUNK = 128 * 128;          // [128 rows x 64 columns] fp16, bytes
 constexpr int P4_TILE = 2 * P4_CHUNK;
-constexpr int P4_SMEM = 6 * P4_TILE + 1024 + 256 * 4 + 256;
-constexpr float P4_LAZY = 8.f;
+constexpr int P4_SMEM = 6 * P4_TILE + 1024 + 256 * 4 + 256 + 256;
+constexpr float P4_P_BIAS = 11.f;
+constexpr float P4_LAZY = 4.f;
 constexpr int P4_PART = HD + 4;              // floats of a row's partial result
 constexpr uint32_t P4_IDESC = (1u << 4) | (128u >> 3) << 17 | (128u >> 4) << 24;   // f16 x f16 -> f32, 128 x 128
 
@@ -69,6 +76,7 @@ enum : int {
   kErrP4O = 0x4405,
   kErrP4KEmpty = 0x4406,
   kErrP4VEmpty = 0x4407,
+  kErrP4Top = 0x4408,
 };
 
 struct Prefill4Args {
@@ -156,13 +164,13 @@ __device__ __forceinline__ P4Tile p4_tile(const Prefill4Args& a, int left) {
 }
 
 // The values s (c + z) of a word's eight codes as four pairs (code i, code i + 4),
-// divided by P4_UNIT: the masked codes are the fp16 subnormals c 2^-24 (c 2^-20),
-// `z` is the zero point times 2^-9 and `s` the scale times 2^5. c + z comes out
-// exactly (it is a multiple of 2^-7 below 16, and finer below 8), so the only
-// rounding is the value's own. Rounding s z once for a whole group instead cost
-// as many instructions and, being the same error for all its channels, moved the
-// scores of long contexts by up to a bf16 step of the output.
-constexpr float P4_UNIT = 16.f;
+// relative to 2^(e - 5), where 2^e is the power of two of the largest scale: the
+// masked codes are the fp16 subnormals c 2^-24 (c 2^-20), `z` is the zero point
+// times 2^-9 and `s` the scale times 2^(14 - e). Two roundings: c + z is exact where
+// the zero point's unit is no finer than the sum's, else off by up to 2^-11 of
+// itself, and the product by as much again. Rounding s z once for a whole group
+// instead cost as many instructions and, being the same error for all its channels,
+// moved the scores of long contexts by up to a bf16 step of the output.
 __device__ __forceinline__ void p4_values(uint32_t w, __half2 s, __half2 z, uint32_t (&v)[4]) {
   const __half2 up0 = __float2half2_rn(32768.f), up1 = __float2half2_rn(2048.f);
 #pragma unroll
@@ -175,10 +183,18 @@ __device__ __forceinline__ void p4_values(uint32_t w, __half2 s, __half2 z, uint
     w >>= 8;
   }
 }
-// A (scale, zero point) word as those two factors: fp16 s 2^5 in the low half, z 2^-9 in the high half.
-__device__ __forceinline__ uint32_t p4_factors(uint32_t word) {
-  return pack_f16(kv4_scale(word) * 32.f, kv4_zero(word) * 0.001953125f);
+// A (scale, zero point) word as those two factors: fp16 s 2^(14 - e) in the low half, z 2^-9 in the high half.
+__device__ __forceinline__ uint32_t p4_factors(uint32_t word, int e) {
+  return pack_f16(kv4_scale(word) * __uint_as_float((uint32_t)(127 + 14 - e) << 23), kv4_zero(word) * 0.001953125f);
 }
+// The exponent of a word's scale, kept where 2^(14 - e) is finite. Scales are
+// below 2^11; what is not one (a NaN) counts as the largest.
+constexpr int P4_E_MIN = -110;
+__device__ __forceinline__ int p4_exponent(uint32_t word) {
+  return min(11, max(P4_E_MIN, (int)(word >> 23 & 255u) - 127));
+}
+// 2^(e - 5): what a stored 1 stands for.
+__device__ __forceinline__ float p4_unit(int e) { return __uint_as_float((uint32_t)(127 - 5 + e) << 23); }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -218,7 +234,13 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
   uint64_t* p_full = bars + 10;   // [2] by tile
   uint64_t* o_done = bars + 12;   // [2] by tile
   uint64_t* drain = bars + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* top_full = bars + 15;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  // Units of the operands, by key tile modulo 4: a slot is written again when the
+  // scores of two tiles later have been taken, by when every softmax has read it.
+  float* k_unit = reinterpret_cast<float*>(bars + 32);   // [4][dequantising warp]
+  float* v_unit = k_unit + 16;                           // [4][group]
+  uint32_t* v_top = reinterpret_cast<uint32_t*>(v_unit + 16);   // [2][group][warp] largest words of a tile
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int kvh = blockIdx.y;
@@ -260,6 +282,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       mbar_init(&o_done[i], 1);
     }
     mbar_init(drain, 1);
+    mbar_init(top_full, 4);
     fence_barrier_init();
   }
   if (warp == 12) tmem_alloc(tmem_slot, 512);
@@ -283,7 +306,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     const int e = min(126, max(-100, (int)((__float_as_uint(amax) >> 23) & 255u) - 127));
     const float up = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (half == 0) sF[r] = a.scale_log2 * P4_UNIT * exp2f((float)e);
+    if (half == 0) sF[r] = a.scale_log2 * exp2f((float)e);
     uint8_t* dst = sQ + (r >> 7) * P4_TILE + half * P4_CHUNK + (r & 127) * 128;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -343,37 +366,53 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
         for (int i = 0; i < 128; ++i)
           if (i >= lim) s[i] = -INFINITY;
       }
-      float red[4];
+      float red[4], fc[4];
+      {
+        const float4 u = *reinterpret_cast<const float4*>(k_unit + (j & 3) * 4);
+        const float uc[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) red[c] = fmaxf(s[2 * c], s[2 * c + 1]);
+        for (int c = 0; c < 4; ++c) fc[c] = fminf(fmaxf(f * uc[c], 1.2e-38f), 3e38f);   // 0 would make a masked key NaN
+      }
 #pragma unroll
-      for (int i = 8; i < 128; i += 2) red[i / 2 & 3] = max3(red[i / 2 & 3], s[i], s[i + 1]);
-      const float row_max = f * fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      // The reference maximum moves only when it is exceeded by 2^8: P stays
-      // below 2^8 in fp16 and the common factor cancels in O / l.
+      for (int c = 0; c < 4; ++c) red[c] = fmaxf(s[32 * c], s[32 * c + 1]);
+#pragma unroll
+      for (int i = 2; i < 32; i += 2)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) red[c] = max3(red[c], s[32 * c + i], s[32 * c + i + 1]);
+      const float row_max = fmaxf(fmaxf(fc[0] * red[0], fc[1] * red[1]), fmaxf(fc[2] * red[2], fc[3] * red[3]));
+      // The reference maximum moves only when it is exceeded by 2^4: P stays
+      // below 2^15 in fp16 and the common factor cancels in O / l.
       const bool move = m == -INFINITY || row_max > m + P4_LAZY;
       const float mx = move ? fmaxf(m, row_max) : m;
       const float corr = m == -INFINITY ? 0.f : (move ? kv4_exp2(m - mx) : 1.f);
-      const float ref = mx == -INFINITY ? 0.f : mx;
+      const float ref = mx == -INFINITY ? 0.f : mx - P4_P_BIAS;
       l *= corr;
       m = mx;
       // s_full of this tile was committed after the last product into O
-      if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+      bool scale_o = corr != 1.f;
+      const uint32_t* unit_now = reinterpret_cast<const uint32_t*>(v_unit) + (j & 3) * 4;
+      const uint32_t* unit_before = reinterpret_cast<const uint32_t*>(v_unit) + (j - 1 & 3) * 4;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) scale_o |= unit_now[i] != unit_before[i];
+      if (j > 0 && __any_sync(0xffffffffu, scale_o)) {
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
+          const int i = c * NG / 8;
+          const float by = corr * __uint_as_float(unit_before[i] - unit_now[i] + (127u << 23));
           uint32_t v[16];
           tmem_ld_x16(t_o + c * 16, v);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+          for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * by);
           tmem_st_x16(t_o + c * 16, v);
         }
       }
-      const float2 f2 = make_float2(f, f), r2 = make_float2(-ref, -ref);
+      const float2 r2 = make_float2(-ref, -ref);
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t p[16];
+        const float2 f2 = make_float2(fc[c], fc[c]);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 e = fma2(make_float2(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), f2, r2);
@@ -390,6 +429,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       mbar_arrive(&p_full[x]);
     }
     if (ok && n > 0) ok = __all_sync(0xffffffffu, kv4_wait(&o_done[x], 0, kErrP4O));
+    const float* unit = v_unit + (n - 1 & 3) * 4;           // of O
     if (ok && a.splits > 1) {
       tc_fence_after();
       float* dst = a.part + ((((size_t)blockIdx.x * a.kv_heads + kvh) * a.splits + blockIdx.z) * 128 + r) * P4_PART;
@@ -401,22 +441,27 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
           uint32_t v[16];
           tmem_ld_x16(t_o + c * 16, v);
           tmem_ld_wait();
+          const float by = unit[c * NG / 8];
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<uint4*>(dst + c * 16 + u * 4) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+            *reinterpret_cast<float4*>(dst + c * 16 + u * 4) =
+                make_float4(__uint_as_float(v[4 * u]) * by, __uint_as_float(v[4 * u + 1]) * by,
+                            __uint_as_float(v[4 * u + 2]) * by, __uint_as_float(v[4 * u + 3]) * by);
         }
       }
     } else if (ok) {
       tc_fence_after();
-      const float inv = l != 0.f ? P4_UNIT / l : 0.f;       // a row that sees no key gives zeros
+      const float inv = l != 0.f ? 1.f / l : 0.f;           // a row that sees no key gives zeros
       __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
                            (int64_t)(kvh * a.group + row % a.group) * HD;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
+        float by = 0.f;
         if (n > 0) {
           tmem_ld_32x32b_x32(t_o + c * 32, v);
           tmem_ld_wait();
+          by = unit[c * NG / 4];
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0;
@@ -427,7 +472,8 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = pack2_bf16(__uint_as_float(v[u * 8 + 2 * e]) * inv, __uint_as_float(v[u * 8 + 2 * e + 1]) * inv);
+              w[e] = pack2_bf16(__uint_as_float(v[u * 8 + 2 * e]) * inv * by,
+                                __uint_as_float(v[u * 8 + 2 * e + 1]) * inv * by);
             *reinterpret_cast<uint4*>(dst + c * 32 + u * 8) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
@@ -476,13 +522,13 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
 #pragma unroll
       for (int i = 0; i < NG; ++i)
         kp[i] = in ? *reinterpret_cast<const uint32_t*>(rec + KV4_CODES + 64 * i + 4 * (lane & 15)) : 0u;
-    };
-    auto load_v = [&]() {
-      const uint8_t* v = rec != nullptr ? rec + kv4_record(NG) : nullptr;
       // a key that no query sees is a zero row whatever its record holds
 #pragma unroll
       for (int i = 0; i < NG; ++i)
-        vp[i] = in ? *reinterpret_cast<const uint32_t*>(v + KV4_CODES + 64 * i + 4 * (lane & 15)) : 0u;
+        vp[i] = in ? *reinterpret_cast<const uint32_t*>(rec + kv4_record(NG) + KV4_CODES + 64 * i + 4 * (lane & 15)) : 0u;
+    };
+    auto load_v = [&]() {
+      const uint8_t* v = rec != nullptr ? rec + kv4_record(NG) : nullptr;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const uint8_t* p = reinterpret_cast<const uint8_t*>(
@@ -492,6 +538,9 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
           vc[b][i] = p != nullptr ? *reinterpret_cast<const uint4*>(p + i * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
       }
     };
+    int ev[NG];                                 // V's exponents, the largest scale so far
+#pragma unroll
+    for (int i = 0; i < NG; ++i) ev[i] = P4_E_MIN;
     if (n_max > 0) {
       if (at_key - (lane & 15) < kv_end) page = tab[at_page];
       next();
@@ -502,11 +551,34 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       const int st = j & 1;
       const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u;
       if (!__all_sync(0xffffffffu, kv4_wait(&k_empty[st], ph, kErrP4KEmpty))) break;
+      // The tile's units. The warps exchange V's largest words through a barrier
+      // whose wait is bounded: one that gave up does not hold the others.
+      uint32_t top = kp[0];
+#pragma unroll
+      for (int i = 1; i < NG; ++i) top = max(top, kp[i]);
+      const int ek = p4_exponent(__reduce_max_sync(0xffffffffu, top));
+      uint32_t* tops = v_top + (j & 1) * 16;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint32_t x = __reduce_max_sync(0xffffffffu, vp[i]);
+        if (lane == 0) tops[4 * i + w4] = x;
+      }
+      if (lane == 0) {
+        k_unit[(j & 3) * 4 + w4] = p4_unit(ek);
+        mbar_arrive(top_full);
+      }
+      if (!__all_sync(0xffffffffu, kv4_wait(top_full, (uint32_t)j & 1u, kErrP4Top))) break;
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(tops + 4 * i);
+        ev[i] = max(ev[i], p4_exponent(max(max(x.x, x.y), max(x.z, x.w))));
+        if (w4 == 0 && lane == 0) v_unit[(j & 3) * 4 + i] = p4_unit(ev[i]);
+      }
       {
         uint8_t* dst = sK + st * P4_TILE + key * 128;
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-          const uint32_t f = p4_factors(kp[i]);
+          const uint32_t f = p4_factors(kp[i], ek);
           const uint32_t f0 = __byte_perm(f, f, 0x1010), f1 = __byte_perm(f, f, 0x3232);
           const __half2 sc = *reinterpret_cast<const __half2*>(&f0), sz = *reinterpret_cast<const __half2*>(&f1);
 #pragma unroll
@@ -524,13 +596,13 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[st]);
+      uint32_t ss[NG];                                      // the factors of this lane's token
+#pragma unroll
+      for (int i = 0; i < NG; ++i) ss[i] = p4_factors(vp[i], ev[i]);
       if (j + 1 < n_max) {
         next();
         load_k();
       }
-      uint32_t ss[NG];                                      // the factors of this lane's token
-#pragma unroll
-      for (int i = 0; i < NG; ++i) ss[i] = p4_factors(vp[i]);
       if (!__all_sync(0xffffffffu, kv4_wait(&v_empty[st], ph, kErrP4VEmpty))) break;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -654,7 +726,7 @@ __global__ void __launch_bounds__(256) prefill4_join_kernel(const Prefill4Args a
     o.z = fmaf(v.z, e, o.z);
     o.w = fmaf(v.w, e, o.w);
   }
-  const float inv = L != 0.f ? P4_UNIT / L : 0.f;
+  const float inv = L != 0.f ? 1.f / L : 0.f;
   __nv_bfloat16* dst = a.out + (int64_t)(q_begin + row / a.group) * a.out_stride +
                        (int64_t)(kvh * a.group + row % a.group) * HD + 4 * lane;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));

@@ -510,7 +510,7 @@ def check_magnitudes(op, q, k, v, page, group, ws, g):
     return p
 
 
-OPS = ["decode"]
+OPS = ["decode", "prefill"]
 
 
 @pytest.mark.parametrize("group", ops.KV4_GROUPS)
