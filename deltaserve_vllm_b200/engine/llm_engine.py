@@ -625,10 +625,11 @@ class CoServingEngine:
             raise KeyError(f"no decoding request {request_id!r}")
         if len(self.scheduler.running) >= self.ecfg.max_num_seqs:
             raise MemoryError("max_num_seqs requests are running")
-        child = Request(new_id, list(r.prompt_ids), params or r.params, r.adapter, status=r.status,
+        # The times go with the tokens: the child's latencies are the parent's up to here.
+        child = Request(new_id, list(r.prompt_ids), params or r.params, r.adapter, r.arrival_time, status=r.status,
                         output_ids=list(r.output_ids), num_computed=r.num_computed, lora_slot=r.lora_slot,
-                        num_cached_tokens=r.num_computed, first_token_time=r.first_token_time,
-                        block_hashes=list(r.block_hashes))
+                        num_cached_tokens=r.num_prompt, first_token_time=r.first_token_time,
+                        token_times=list(r.token_times), block_hashes=list(r.block_hashes))
         child.output_logprobs = list(r.output_logprobs)
         child.output_top_logprobs = list(r.output_top_logprobs)
         with torch.cuda.stream(self.fwd_stream):  # behind the last forward, ahead of the next

@@ -206,3 +206,22 @@ def test_fork_and_compact_copy_on_the_forward_stream(monkeypatch):
     eng.scheduler.abort("r1")                     # leaves holes for the compaction
     eng.compact_kv()
     assert [s for s, _ in copied] == ["forward"] * 2 and all(n for _, n in copied)
+
+
+def test_a_forks_timeline_is_its_tokens():
+    """A fork carries its parent's tokens and their times: no time runs backwards, no gap spans several tokens."""
+    eng = engine()
+    for i, p in enumerate(prompts(2)):
+        eng.add_request(f"r{i}", p, SamplingParams(max_tokens=8))
+    while len(eng.requests["r1"].output_ids) < 5:
+        eng.step()
+    r = eng.requests["r1"]
+    child = eng.fork_request("r1", "fork")
+    assert child.ttft() == r.ttft() > 0
+    assert child.num_cached_tokens == child.num_prompt
+    eng.run_until_idle(max_steps=50)
+    for x in (r, child):
+        assert len(x.tbts()) == len(x.output_ids) - 1 == 7
+        assert all(t >= 0 for t in x.tbts())
+    assert child.tbts()[:4] == r.tbts()[:4] and child.token_times is not r.token_times
+    assert child.finish_time - child.arrival_time >= child.ttft() + sum(child.tbts())
