@@ -614,8 +614,9 @@ class CoServingEngine:
 
     def fork_request(self, request_id: str, new_id: str, params: SamplingParams | None = None) -> Request:
         """A copy of a decoding request that goes on by itself from the same
-        tokens (with ``params``, e.g. another seed): full KV pages are shared,
-        the partly filled one is copied. Single rank only."""
+        tokens (with ``params``, e.g. another seed; ``max_tokens`` counts the
+        tokens produced so far): full KV pages are shared, the partly filled one
+        is copied. Single rank only."""
         if self.tp_size > 1:
             raise ValueError("fork_request needs tensor_parallel_size 1")
         if new_id in self.requests:
@@ -625,8 +626,13 @@ class CoServingEngine:
             raise KeyError(f"no decoding request {request_id!r}")
         if len(self.scheduler.running) >= self.ecfg.max_num_seqs:
             raise MemoryError("max_num_seqs requests are running")
+        params = params or r.params
+        if params.max_tokens <= len(r.output_ids):
+            raise ValueError(f"max_tokens {params.max_tokens}: {request_id!r} has produced {len(r.output_ids)} tokens")
+        if r.num_prompt + params.max_tokens > self.scheduler.max_model_len:
+            raise ValueError(f"prompt + max_tokens exceeds max_model_len={self.scheduler.max_model_len}")
         # The times go with the tokens: the child's latencies are the parent's up to here.
-        child = Request(new_id, list(r.prompt_ids), params or r.params, r.adapter, r.arrival_time, status=r.status,
+        child = Request(new_id, list(r.prompt_ids), params, r.adapter, r.arrival_time, status=r.status,
                         output_ids=list(r.output_ids), num_computed=r.num_computed, lora_slot=r.lora_slot,
                         num_cached_tokens=r.num_prompt, first_token_time=r.first_token_time,
                         token_times=list(r.token_times), block_hashes=list(r.block_hashes))

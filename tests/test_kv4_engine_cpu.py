@@ -225,3 +225,21 @@ def test_a_forks_timeline_is_its_tokens():
         assert all(t >= 0 for t in x.tbts())
     assert child.tbts()[:4] == r.tbts()[:4] and child.token_times is not r.token_times
     assert child.finish_time - child.arrival_time >= child.ttft() + sum(child.tbts())
+
+
+def test_a_fork_has_tokens_left_to_produce():
+    """A fork's parameters allow at least one more token, within the model's length; a refused fork changes nothing."""
+    eng = engine()
+    eng.add_request("a", prompts(2)[1], SamplingParams(max_tokens=8))
+    while len(eng.requests["a"].output_ids) < 4:
+        eng.step()
+    free, block_ids = eng.kv.allocator.num_free, list(eng.requests["a"].block_ids)
+    for n in (0, 2, 4, 256 - 26 + 1):
+        with pytest.raises(ValueError):
+            eng.fork_request("a", "b", SamplingParams(max_tokens=n))
+    assert eng.kv.allocator.num_free == free and eng.requests["a"].block_ids == block_ids and "b" not in eng.requests
+    child = eng.fork_request("a", "b", SamplingParams(max_tokens=5))
+    longest = eng.fork_request("a", "c", SamplingParams(max_tokens=256 - 26))
+    eng.run_until_idle(max_steps=500)
+    assert len(child.output_ids) == 5 and len(longest.output_ids) == 256 - 26
+    assert eng.kv.allocator.num_free == eng.kv.allocator.num_blocks
