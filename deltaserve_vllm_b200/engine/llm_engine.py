@@ -631,6 +631,9 @@ class CoServingEngine:
             raise ValueError(f"max_tokens {params.max_tokens}: {request_id!r} has produced {len(r.output_ids)} tokens")
         if r.num_prompt + params.max_tokens > self.scheduler.max_model_len:
             raise ValueError(f"prompt + max_tokens exceeds max_model_len={self.scheduler.max_model_len}")
+        if (params.logprobs and not r.params.logprobs) or \
+                (params.logprobs and params.top_logprobs and not r.params.top_logprobs):
+            raise ValueError(f"{request_id!r} has no log-probabilities of its tokens so far")
         # The times go with the tokens: the child's latencies are the parent's up to here.
         child = Request(new_id, list(r.prompt_ids), params, r.adapter, r.arrival_time, status=r.status,
                         output_ids=list(r.output_ids), num_computed=r.num_computed, lora_slot=r.lora_slot,

@@ -243,3 +243,23 @@ def test_a_fork_has_tokens_left_to_produce():
     eng.run_until_idle(max_steps=500)
     assert len(child.output_ids) == 5 and len(longest.output_ids) == 256 - 26
     assert eng.kv.allocator.num_free == eng.kv.allocator.num_blocks
+
+
+@pytest.mark.parametrize("parent,child,ok", [({}, dict(logprobs=True), False),
+                                             (dict(logprobs=True), dict(logprobs=True, top_logprobs=2), False),
+                                             (dict(logprobs=True, top_logprobs=2), dict(logprobs=True, top_logprobs=1), True),
+                                             (dict(logprobs=True), {}, True)])
+def test_a_forks_logprobs_are_its_tokens(parent, child, ok):
+    """Log-probabilities are read by the token's position: a fork can only go on with those that its parent recorded."""
+    eng = engine()
+    eng.add_request("a", prompts(1)[0], SamplingParams(max_tokens=6, **parent))
+    while len(eng.requests["a"].output_ids) < 3:
+        eng.step()
+    if not ok:
+        with pytest.raises(ValueError):
+            eng.fork_request("a", "b", SamplingParams(max_tokens=6, **child))
+        return
+    r = eng.fork_request("a", "b", SamplingParams(max_tokens=6, **child))
+    eng.run_until_idle(max_steps=50)
+    if r.params.logprobs:
+        assert len(r.output_logprobs) == 6 and (not r.params.top_logprobs or len(r.output_top_logprobs) == 6)
