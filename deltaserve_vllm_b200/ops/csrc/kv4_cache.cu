@@ -367,6 +367,8 @@ int dsv_kv4_groups(const torch::Tensor& cache, const char* op) {
                     op, ": cache must be a CUDA uint8 tensor [pages, kv heads, page size / 16, 2, record bytes]");
   TORCH_CHECK_VALUE(cache.is_contiguous() && reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, op,
                     ": cache must be contiguous and 16-byte aligned");
+  TORCH_CHECK_VALUE(cache.size(0) > 0 && cache.size(1) > 0 && cache.size(2) > 0, op,
+                    ": cache has no pages, no kv heads or no 16-token records");
   const int64_t rec = cache.size(4);
   const int ng = rec == dsv::kv4_record(1) ? 1 : rec == dsv::kv4_record(2) ? 2 : rec == dsv::kv4_record(4) ? 4 : 0;
   TORCH_CHECK_VALUE(ng != 0, op, ": record of ", std::to_string(rec), " bytes is none of 1088, 1152, 1280 (groups of 128, 64, 32)");

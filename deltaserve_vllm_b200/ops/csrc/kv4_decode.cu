@@ -329,6 +329,9 @@ int64_t dsv_paged_decode4(torch::Tensor q, torch::Tensor cache, torch::Tensor ta
                         ctx.scalar_type() == at::kInt && ctx.dim() == 1 && ctx.size(0) == B && ctx.is_contiguous() &&
                         tables.device() == cache.device() && ctx.device() == cache.device(),
                     "paged_decode4: block tables must be int32 [batch, pages], context lengths int32 [batch]");
+  const int64_t most = tables.size(1) * cache.size(2) * 16;     // longest context
+  TORCH_CHECK_VALUE(most < (int64_t(1) << 31) && B * hkv * (most / 32 + 1) < (int64_t(1) << 31),
+                    "paged_decode4: block tables of more than 2^31 tokens");
   TORCH_CHECK_VALUE(ws.is_cuda() && ws.device() == cache.device() && ws.is_contiguous() &&
                         (int64_t)ws.nbytes() >= dsv_kv4_workspace_bytes(),
                     "paged_decode4: the workspace must come from kv4_workspace on the cache's device");

@@ -772,6 +772,8 @@ int64_t dsv_paged_prefill4(torch::Tensor q, torch::Tensor cache, torch::Tensor t
   TORCH_CHECK_VALUE(tables.scalar_type() == at::kInt && tables.dim() == 2 && tables.size(0) == ctx.size(0) &&
                         tables.is_contiguous() && tables.device() == cache.device(),
                     "paged_prefill4: block tables must be int32 [sequences, pages]");
+  TORCH_CHECK_VALUE(tables.size(1) * cache.size(2) * 16 < (int64_t(1) << 31) && hkv < 65536,
+                    "paged_prefill4: block tables of more than 2^31 tokens, or more than 65535 kv heads");
   TORCH_CHECK_VALUE(ws.is_cuda() && ws.device() == cache.device() && ws.is_contiguous() &&
                         (int64_t)ws.nbytes() >= dsv_kv4_workspace_bytes(),
                     "paged_prefill4: the workspace must come from kv4_workspace on the cache's device");

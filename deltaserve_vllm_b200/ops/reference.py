@@ -159,6 +159,8 @@ KV4_TINY = 2.0 ** -120
 def _kv4_group(cache) -> int:
     if cache.dtype != torch.uint8 or cache.dim() != 5 or cache.shape[3] != 2:
         raise ValueError("kv4 cache must be uint8 [pages, kv heads, page size / 16, 2, record bytes]")
+    if not min(cache.shape):
+        raise ValueError("kv4 cache has no pages, no kv heads or no 16-token records")
     for group in (32, 64, 128):
         if cache.shape[4] == 1024 + 64 * (128 // group):
             return group
@@ -247,8 +249,8 @@ def _kv4_pages(cache, block_table, ctx):
 
 def paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale):
     _kv4_group(cache)
-    if num_heads % cache.shape[1]:
-        raise ValueError("query heads must be a multiple of the kv heads")
+    if num_heads <= 0 or num_heads % cache.shape[1] or num_heads // cache.shape[1] > 16:
+        raise ValueError("query heads must be 1 to 16 times the kv heads")
     for s in range(ctx_lens.shape[0]):
         q0, q1, ctx = int(cu_q[s]), int(cu_q[s + 1]), int(ctx_lens[s])
         if ctx == 0:

@@ -120,3 +120,27 @@ def test_refusals():
                                           torch.zeros(1, 384), 3, 1.0, None)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("shape", [(0, 1, 1), (2, 0, 1), (2, 1, 0)])
+def test_an_empty_cache_is_refused(shape):
+    cache = torch.zeros(*shape, 2, 1152, dtype=torch.uint8)
+    q, one, cu = torch.zeros(1, 128), torch.ones(1, dtype=torch.int32), torch.arange(2, dtype=torch.int32)
+    tables, slots = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)
+    k = torch.zeros(1, shape[1] * 128, dtype=torch.bfloat16)
+    for call in (lambda: ops.kv4_write(k, k, cache, slots), lambda: ops.kv4_read(cache, slots),
+                 lambda: ops.paged_decode4(q, cache, tables, one, q.clone(), 1, 1.0, None),
+                 lambda: ops.paged_prefill4(q, cache, tables, cu, one, q.clone(), 1, 1.0, None)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("heads", [0, 17, 32])
+def test_query_heads_are_1_to_16_times_the_kv_heads(heads):
+    cache = torch.zeros(ops.kv4_cache_shape(1, 1, 16, 64), dtype=torch.uint8)
+    q, one, cu = torch.zeros(1, heads * 128), torch.ones(1, dtype=torch.int32), torch.arange(2, dtype=torch.int32)
+    tables = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.paged_decode4(q, cache, tables, one, q.clone(), heads, 1.0, None)
+    with pytest.raises(ValueError):
+        ops.paged_prefill4(q, cache, tables, cu, one, q.clone(), heads, 1.0, None)

@@ -642,6 +642,32 @@ def test_refusals(ws):
         ops.paged_decode4(wide, cache, tables, ctx, torch.empty_like(wide), 34, SCALE, ws)
 
 
+@pytest.mark.parametrize("shape", [(0, 1, 1), (2, 0, 1), (2, 1, 0)])
+def test_an_empty_cache_is_refused(shape, ws):
+    cache = torch.zeros(*shape, 2, 1152, dtype=torch.uint8, device=DEV)
+    q = torch.zeros(1, 128, dtype=torch.bfloat16, device=DEV)
+    one, cu = torch.ones(1, dtype=torch.int32, device=DEV), torch.arange(2, dtype=torch.int32, device=DEV)
+    tables, slots = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    k = torch.zeros(1, shape[1] * 128, dtype=torch.bfloat16, device=DEV)
+    for call in (lambda: ops.kv4_write(k, k, cache, slots), lambda: ops.kv4_read(cache, slots),
+                 lambda: ops.paged_decode4(q, cache, tables, one, q.clone(), 1, 1.0, ws),
+                 lambda: ops.paged_prefill4(q, cache, tables, cu, one, q.clone(), 1, 1.0, ws)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_tables_of_too_many_tokens_are_refused(ws):
+    """The token count of a table row is 32 bits."""
+    cache = empty_cache(1, 1, 1 << 16, 64)
+    q = torch.zeros(1, 128, dtype=torch.bfloat16, device=DEV)
+    one, cu = torch.ones(1, dtype=torch.int32, device=DEV), torch.arange(2, dtype=torch.int32, device=DEV)
+    tables = torch.zeros(1, 1 << 15, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        ops.paged_decode4(q, cache, tables, one, q.clone(), 1, SCALE, ws)
+    with pytest.raises(ValueError):
+        ops.paged_prefill4(q, cache, tables, cu, one, q.clone(), 1, SCALE, ws)
+
+
 def test_copy_refusals():
     caches = [empty_cache(4, 1, 16, 64) for _ in range(2)]
     for src, dst in (([0], [1, 2]), ([0], [4]), ([-1], [0]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0], [0])):
