@@ -139,13 +139,15 @@ struct P4Tile {
   int seq, local;           // sequence (-1: past the last tile) and which of its query tiles
 };
 // The `left`-th tile of the packed sequences: a sequence's last, longest tile first.
+// A sequence whose rows are not rows of q has none, and is an error.
 __device__ __forceinline__ P4Tile p4_tile(const Prefill4Args& a, int left) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < a.seqs; s0 += 32) {
     int n = 0;
     if (s0 + lane < a.seqs) {
-      const int len = a.cu_q[s0 + lane + 1] - a.cu_q[s0 + lane];
-      n = len > 0 ? (len * a.group + a.tile_rows - 1) / a.tile_rows : 0;
+      const int begin = a.cu_q[s0 + lane], end = a.cu_q[s0 + lane + 1];
+      if (begin < 0 || end < begin || end > a.rows) set_error(kErrShape);
+      else n = ((end - begin) * a.group + a.tile_rows - 1) / a.tile_rows;
     }
     int up = n;
 #pragma unroll

@@ -461,6 +461,28 @@ def test_prefill_page_outside_the_cache_is_an_error(ws):
     assert ops.check_device_error() != 0
 
 
+@pytest.mark.parametrize("offsets", [[0, 40, 300], [-7, 40, 100], [0, 90, 60], [200, 240, 300], [0, 40, 1 << 30]])
+def test_prefill_offsets_outside_the_rows_are_an_error(offsets, ws):
+    """No row outside q is read or written; the sequences that are inside are answered."""
+    g = gen(25)
+    cache, tables, values = filled(g, [50, 60], 2, 16, 64)
+    ctx = torch.tensor([50, 60], dtype=torch.int32, device=DEV)
+    base = torch.randn(400, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    q, outs = base[100:200], torch.full((400, 4 * 128), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.paged_prefill4(q, cache, tables, torch.tensor(offsets, dtype=torch.int32, device=DEV), ctx, outs[100:200], 4, SCALE, ws)
+    assert ops.check_device_error() != 0
+    assert bool((outs[:100] == 7).all()) and bool((outs[200:] == 7).all())
+    for i, n in enumerate((50, 60)):
+        lo, hi = offsets[i], offsets[i + 1]
+        if 0 <= lo <= hi <= 100:
+            seen = torch.arange(n, device=DEV)[None] <= n - (hi - lo) + torch.arange(hi - lo, device=DEV)[:, None]
+            live = seen.any(1)
+            exp = attention64(q[lo:hi][live].reshape(-1, 4, 128), *values[i], seen[live])
+            assert bool(((outs[100 + lo:100 + hi][live].double() - exp).abs() <= exp.abs() * 2 ** -8 +
+                         float(values[i][1].abs().max()) * 2 ** -7).all())
+            assert bool((outs[100 + lo:100 + hi][~live] == 0).all())
+
+
 # ----------------------------------------------------------------- magnitudes
 
 def held(g, k, v, page, group):
