@@ -147,10 +147,13 @@ __global__ void __launch_bounds__(D4_WARPS * 32, MIN_CTAS) decode4_kernel(const 
   uint64_t* full = full_bars[warp];
   int* pages = page_ids[warp];
 
-  // Sequences without context give zeros.
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
+  // Sequences without context give zeros; one longer than its table is an error
+  // (only those pages are seen).
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (a.ctx[b] > a.max_pages * a.sub * 16 && threadIdx.x == 0) set_error(kErrShape);
     if (a.ctx[b] <= 0 || a.max_pages == 0)
       for (int i = threadIdx.x; i < a.heads * HD; i += D4_WARPS * 32) a.out[b * a.out_stride + i] = f2bf(0.f);
+  }
 
   const int total = d4_total(a);
   const int runs = (int)gridDim.x * D4_WARPS;

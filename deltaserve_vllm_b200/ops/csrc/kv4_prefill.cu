@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
   const int kv_end = pos0 + (row0 + rows - 1) / a.group + 1;
 
   if (threadIdx.x == 0) {
+    if (a.ctx[seq] > ctx) set_error(kErrShape);           // longer than its table: only those pages are seen
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 128);
       mbar_init(&v_full[i], 128);

@@ -483,6 +483,25 @@ def test_prefill_offsets_outside_the_rows_are_an_error(offsets, ws):
             assert bool((outs[100 + lo:100 + hi][~live] == 0).all())
 
 
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+def test_a_context_longer_than_its_table_is_an_error(op, ws):
+    g = gen(26)
+    cache, tables, values = filled(g, [40, 50], 2, 16, 64, extra_cols=0)       # 4 pages a row
+    q = torch.randn(2, 4 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    def call(ctx):
+        ctx = torch.tensor(ctx, dtype=torch.int32, device=DEV)
+        if op == "decode":
+            return ops.paged_decode4(q, cache, tables, ctx, out, 4, SCALE, ws).clone()
+        cu = torch.arange(3, dtype=torch.int32, device=DEV)
+        return ops.paged_prefill4(q, cache, tables, cu, ctx, out, 4, SCALE, ws).clone()
+    exp = call([40, 50])
+    assert ops.check_device_error() == 0
+    got = call([40, 65])
+    assert ops.check_device_error() != 0
+    assert torch.equal(got[0], exp[0])
+
+
 # ----------------------------------------------------------------- magnitudes
 
 def held(g, k, v, page, group):
