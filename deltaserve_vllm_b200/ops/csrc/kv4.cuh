@@ -75,12 +75,27 @@ __device__ __forceinline__ float kv4_exp2(float x) {
   return y;
 }
 
-// mbar_wait that polls a while before its limit's clock is read: these kernels'
-// stages turn over in well under a microsecond.
+// Bounded wait as mbar_wait, but for two things: it polls a while before its
+// limit's clock is read (these kernels' stages turn over in well under a
+// microsecond), and a recorded kErrShape does not end it. That one says that an
+// index of some call was out of range and not followed; the waits still complete,
+// and the other sequences their results.
 __device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity, int code) {
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, code);
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 1023u) == 0) {
+      const int seen = *(volatile int*)&g_error;
+      if (seen != 0 && seen != kErrShape) return false;
+      if (globaltimer_ns() - t0 > kWaitNs) {
+        if (seen != 0) atomicCAS(&g_error, kErrShape, code);
+        else set_error(code);
+        return false;
+      }
+    }
+  }
 }
 
 // Bounded wait that goes on when another wait has given up: for what must end

@@ -502,6 +502,27 @@ def test_a_context_longer_than_its_table_is_an_error(op, ws):
     assert torch.equal(got[0], exp[0])
 
 
+@pytest.mark.parametrize("op", ["decode", "prefill"])
+def test_one_bad_page_spoils_its_own_sequence_only(op, ws):
+    """An index that was not followed stays in the error word until it is read; calls meanwhile wait as long as they need."""
+    g = gen(27)
+    contexts = [40] + [3000] * 40
+    cache, tables, _ = filled(g, contexts, 2, 64, 64, extra_cols=0)
+    ctx = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    cu = torch.arange(42, dtype=torch.int32, device=DEV)
+    q = torch.randn(41, 8 * 128, generator=g, device=DEV).to(torch.bfloat16)
+    def call(tables):
+        if op == "decode":
+            return ops.paged_decode4(q, cache, tables, ctx, torch.empty_like(q), 8, SCALE, ws)
+        return ops.paged_prefill4(q, cache, tables, cu, ctx, torch.empty_like(q), 8, SCALE, ws)
+    exp, bad = call(tables), tables.clone()
+    bad[0, 0] = 1 << 20
+    assert torch.equal(call(bad)[1:], exp[1:])
+    for _ in range(20):                      # the error has not been read
+        assert torch.equal(call(tables), exp)
+    assert ops.check_device_error() == 6     # an index out of range, no wait that gave up
+
+
 # ----------------------------------------------------------------- magnitudes
 
 def held(g, k, v, page, group):
