@@ -26,8 +26,8 @@
 // that of the largest scale of a warp's 32 keys (undone on the score), V to that of
 // the largest scale so far of each group of channels (a larger one rescales O, as a
 // larger maximum does), each query row to that of its largest magnitude, and P to a
-// reference that puts the largest weight between 2^11 and 2^15. A value keeps its
-// bits down to 2^-24 of the largest, a weight to 2^-25. (With fixed divisors of 16
+// reference that puts the largest weight between 2^9 and 2^15. A value keeps its
+// bits down to 2^-24 of the largest, a weight to 2^-23. (With fixed divisors of 16
 // values near 1e-5 were off by 3 %, and weights of 2^-16 beside a dominant key by
 // their rounding to subnormals.)
 //
@@ -63,8 +63,8 @@ constexpr int P4_THREADS = 512;
 constexpr int P4_CHUNK = 128 * 128;          // [128 rows x 64 columns] fp16, bytes
 constexpr int P4_TILE = 2 * P4_CHUNK;
 constexpr int P4_SMEM = 6 * P4_TILE + 1024 + 256 * 4 + 256 + 256;
-constexpr float P4_P_BIAS = 11.f;
-constexpr float P4_LAZY = 4.f;
+constexpr float P4_P_BIAS = 9.f;
+constexpr float P4_LAZY = 6.f;                // 4: 12 packed sequences 271 us in place of 261, 8 and a bias of 7: 259
 constexpr int P4_PART = HD + 4;              // floats of a row's partial result
 constexpr uint32_t P4_IDESC = (1u << 4) | (128u >> 3) << 17 | (128u >> 4) << 24;   // f16 x f16 -> f32, 128 x 128
 
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(P4_THREADS, 1) prefill4_kernel(const Prefill4A
 #pragma unroll
         for (int c = 0; c < 4; ++c) red[c] = max3(red[c], s[32 * c + i], s[32 * c + i + 1]);
       const float row_max = fmaxf(fmaxf(fc[0] * red[0], fc[1] * red[1]), fmaxf(fc[2] * red[2], fc[3] * red[3]));
-      // The reference maximum moves only when it is exceeded by 2^4: P stays
+      // The reference maximum moves only when it is exceeded by 2^6: P stays
       // below 2^15 in fp16 and the common factor cancels in O / l.
       const bool move = m == -INFINITY || row_max > m + P4_LAZY;
       const float mx = move ? fmaxf(m, row_max) : m;
