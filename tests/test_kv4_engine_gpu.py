@@ -170,3 +170,45 @@ def test_compact_behind_a_running_chunk(dtype):
         eng.run_until_idle(max_steps=500)
         return r1.output_ids
     assert run(True) == run(False)
+
+
+def test_a_mixed_batch_attends_as_on_the_cpu():
+    """Decode, prefill and finetuning rows of one batch over the same codes: the model's attention on both devices.
+
+    bf16 results (2^-8), and as many as the kernels' roundings move an average of values: 2^-7 of the largest."""
+    from deltaserve_vllm_b200.models.decoder import ForwardBatch
+    arch = PRESETS["qwen3-test"]
+    g = torch.Generator().manual_seed(5)
+    hq, hkv, page = arch.num_heads, arch.num_kv_heads, 64
+    dec, new, old, ft = [1, 70, 300], [5, 130], [200, 0], [40, 17]
+    contexts = dec + [a + b for a, b in zip(new, old)]
+    need = [-(-c // page) for c in contexts]
+    perm = torch.randperm(sum(need) + 3, generator=g).tolist()
+    tables = torch.zeros(5, max(need), dtype=torch.int32)
+    cache = torch.zeros(ops.kv4_cache_shape(len(perm), hkv, page, 64), dtype=torch.uint8)
+    for i, c in enumerate(contexts):
+        mine = [perm.pop() for _ in range(need[i])]
+        tables[i, :need[i]] = torch.tensor(mine, dtype=torch.int32)
+        slots = torch.tensor([mine[p // page] * page + p % page for p in range(c)])
+        ops.kv4_write(torch.randn(c, hkv * 128, generator=g), torch.randn(c, hkv * 128, generator=g), cache, slots)
+    lo = len(dec) + sum(new)
+    qkv = torch.randn(lo + sum(ft), (hq + 2 * hkv) * 128, generator=g).to(torch.bfloat16)
+    starts = torch.tensor([0] + ft).cumsum(0)[:-1].tolist()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)
+
+    def run(dev, dt):
+        model = DecoderModel(init_weights(arch, seed=1, device="cpu", dtype=torch.float32).to(dev, dt),
+                             [cache.to(dev)], [], None)
+        b = ForwardBatch(input_ids=None, positions=None, slot_mapping=None, num_decode=len(dec),
+                         dec_block_tables=tables[:3].to(dev), dec_ctx_lens=i32(dec).to(dev), num_prefill_seqs=2,
+                         pf_cu_q=i32([0, new[0], sum(new)]).to(dev), pf_ctx_lens=i32(contexts[3:]).to(dev),
+                         pf_block_tables=tables[3:].contiguous().to(dev),
+                         ft_attn_tiles=ops.dense_attn_tiles(starts, ft, dev, bm=128), ft_lo=lo, ft_hi=lo + sum(ft))
+        out = torch.full((lo + sum(ft), hq * 128), float("nan"), device=dev, dtype=dt)
+        model.attention(0, qkv.to(dev, dt), out, b)
+        return out.float().cpu()
+    a, b = run("cuda", torch.bfloat16), run("cpu", torch.float32)
+    assert ops.check_device_error() == 0
+    assert bool(((a - b).abs() <= b.abs() * 2 ** -8 + float(qkv.abs().max()) * 2 ** -7).all()), float((a - b).abs().max())
+    rel = (a - b).norm(dim=1) / b.norm(dim=1)
+    assert bool((rel <= 2 ** -7).all()), rel.max()
