@@ -242,7 +242,7 @@ class KVCache:
     def compact(self, tables: list[list[int]]) -> int:
         """Move the pages in use to the front of the pool, in one launch, and
         rewrite ``tables`` (every list of page ids that is held, in place).
-        Returns the pages in use: the rest of the pool is free."""
+        Returns the pages in use (cached prefixes are): the rest of the pool is free."""
         moves = self.allocator.compact()
         ops.copy_pages(self.k + self.v, [a for a, _ in moves], [b for _, b in moves])
         to = dict(moves)

@@ -652,7 +652,7 @@ class CoServingEngine:
 
     def compact_kv(self) -> int:
         """Move the KV pages in use to the front of the pool (between steps).
-        Returns how many are in use. Single rank only."""
+        Returns how many are in use (cached prefixes are). Single rank only."""
         if self.tp_size > 1:
             raise ValueError("compact_kv needs tensor_parallel_size 1")
         held = list(self.scheduler.running) + list(self.scheduler.waiting)

@@ -301,7 +301,9 @@ def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws):
     128]`` (row strides free; ``q`` rows 16-byte aligned), ``block_tables`` int32
     ``[B, pages]``, ``ctx_lens`` int32 ``[B]`` (0: zeros out), 1 to 16 query heads
     per KV head. Lengths are read on the device, so a captured call serves any.
-    ``ws`` from :func:`kv4_workspace`."""
+    A page outside the cache, or a length past its table, is not followed and
+    sets the error word (:func:`check_device_error`). ``ws`` from
+    :func:`kv4_workspace`."""
     if cache.is_cuda:
         LAUNCHES[0] += _native(0).paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale, ws)
         return out
@@ -313,7 +315,9 @@ def paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale
     sequences (``cu_q`` int32 ``[S + 1]``: their offsets in ``q`` / ``out``, bf16
     ``[T, Hq * 128]`` with 16-byte aligned rows) against ``ctx_lens`` cached
     tokens each, the new ones among them and last. Tiles are found on the device:
-    no tile list. ``ws`` from :func:`kv4_workspace`."""
+    no tile list. Offsets outside ``q``, a page outside the cache, or a length past
+    its table are not followed and set the error word. ``ws`` from
+    :func:`kv4_workspace`."""
     if cache.is_cuda:
         LAUNCHES[0] += _native(0).paged_prefill4(q, cache, block_tables, cu_q, ctx_lens, out, num_heads, scale, ws)
         return out

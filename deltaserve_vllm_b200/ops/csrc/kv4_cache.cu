@@ -10,8 +10,12 @@
 
 namespace dsv {
 
-// Rows x heads from which records are assembled (rows of 8 heads, one by one
-// against by records: 2048 rows 9.4 / 11.5 us, 8192 rows 31.5 / 25.1 us).
+// Rows x heads from which records are assembled. One by one against by records, us:
+//   rows x heads   1 head        2 heads       8 heads
+//    8192           5.5 /  7.4    5.7 /  7.8    5.7 /  7.5
+//   16384           9.3 / 10.5    9.4 / 10.9    9.7 /  9.2
+//   32768          16.8 / 15.2   16.8 / 15.4   17.0 / 14.2
+//   65536          31.2 / 25.1   31.2 / 25.0   31.2 / 23.4
 constexpr int64_t KV4_MANY = 32768;
 
 struct Kv4RowsArgs {

@@ -19,9 +19,10 @@
 // the order of arrival.
 //
 // Measured against the HBM time of the cache bytes (6.54 TB/s): batch 200 x 4096,
-// 32 / 8 heads, groups of 64: 176 us, 5.4 TB/s (one record per step in place of
-// two: 4.5); 16 x 32768, 64 / 8 heads: 125 us. There about 260 instructions per
-// 16 tokens and their latencies bound it (issue slots 56 % busy, ALU 51 %). Short
+// 32 / 8 heads, groups of 64: 184 us, 5.2 TB/s (one record per step in place of
+// two was a sixth slower); 16 x 32768, 64 / 8 heads, groups of 128: 114 us in a
+// graph, 5.0 TB/s. There about 240 instructions per 16 tokens and their latencies
+// bound it (issue slots and ALU 53 % busy, matrix instructions 29 %). Short
 // contexts are bound by a segment's fixed chain of about 2 us (queries, last
 // partial sums, store) and a join's 3 us (release, counter, two rounds of loads).
 // At least two pieces a run: 1 measured 9.9, 2 7.6 and 4 10.5 us at 64 x 64 tokens.

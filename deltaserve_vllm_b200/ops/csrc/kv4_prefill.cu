@@ -37,14 +37,15 @@
 // the order of the eight channels of a 16-byte unit is that of the pairs
 // (0, 4, 1, 5, 2, 6, 3, 7), and Q is stored in the same order.
 //
-// Shared memory: Q 64 KB, K 2 x 32 KB, V 2 x 32 KB. TMEM: S0, S1, O0, O1 of 128
+// Shared memory: Q 64 KB, K 2 x 32 KB, V 2 x 32 KB, units and factors. TMEM: S0, S1, O0, O1 of 128
 // columns each; P_x takes the first 64 columns of S_x.
 //
-// Measured (32 / 8 heads, groups of 64): 2048 tokens after 29952 in 1388 us,
-// 749 TFLOP/s. Its 256 CTAs are two rounds of 148 (86 % of the SMs' time); in a
+// Measured (32 / 8 heads, groups of 64): 2048 tokens after 29952 in 1250 us,
+// 833 TFLOP/s. Its 256 CTAs are two rounds of 148 (86 % of the SMs' time); in a
 // CTA the products (2048 cycles per 128 keys at full rate), the exponentials (2048
 // at 16 a cycle) and the operands' shared-memory traffic (about 2048) overlap only
-// in part, and with the conversions taken out an earlier step at 709 ran at 955.
+// in part (tensor pipe 56 % busy, exponentials 44 %), and with the conversions
+// taken out an earlier step at 709 ran at 955.
 //
 // Every wait is bounded (common.cuh).
 #include <torch/extension.h>
