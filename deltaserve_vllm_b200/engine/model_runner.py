@@ -379,7 +379,7 @@ class ModelRunner:
         if own_rows:
             lens = [s.num_new for s in out.ft]
             starts = np.cumsum([0] + lens[:-1]).tolist()
-            pk.add("ft_tiles", ops.dense_attn_tiles(starts, lens, "cpu", bm=128).numpy().reshape(-1))
+            pk.add("ft_tiles", ops.dense_attn_tiles(starts, lens, "cpu", bm=128 if ops.ATTN_TC else 64).numpy().reshape(-1))
         if pf:
             btab = np.zeros((len(pf), maxb), dtype=np.int64)
             cu = [0]

@@ -60,7 +60,7 @@ class ForwardBatch:
     pf_tile_info: torch.Tensor | None = None       # [tiles, 2] int32
     # 4-bit cache: FT samples attend to their own rows, not to the cache. The
     # prefill fields then hold the inference sequences only.
-    ft_attn_tiles: torch.Tensor | None = None      # [tiles, 3] int32, rows relative to ft_lo
+    ft_attn_tiles: torch.Tensor | None = None      # [tiles, 3] int32 of 128 rows (without ops.ATTN_TC 64), relative to ft_lo
     slot_ids: torch.Tensor | None = None           # [T] int32 LoRA slot per token (-1 none)
     tile_slots: torch.Tensor | None = None         # [ceil(T/128)] int32 slot bitmask per M tile
     logits_idx: torch.Tensor | None = None         # [R] int64 rows whose logits are needed
@@ -218,8 +218,8 @@ class DecoderModel:
         if b.ft_attn_tiles is not None:
             rows = qkv[hi:].unflatten(1, (-1, self.arch.head_dim))
             k0, v0 = self.hq_l, self.hq_l + self.hkv_l
-            ops.attn_fwd_dense(rows[:, :k0], rows[:, k0:v0], rows[:, v0:], None, self.scale, ctx[hi:],
-                               tiles128=b.ft_attn_tiles)
+            ops.attn_fwd_dense(rows[:, :k0], rows[:, k0:v0], rows[:, v0:], b.ft_attn_tiles, self.scale, ctx[hi:],
+                               tiles128=b.ft_attn_tiles if ops.ATTN_TC else None)
 
     # ------------------------------------------------------------------ forward
     @torch.no_grad()

@@ -172,11 +172,13 @@ def test_compact_behind_a_running_chunk(dtype):
     assert run(True) == run(False)
 
 
-def test_a_mixed_batch_attends_as_on_the_cpu():
+@pytest.mark.parametrize("tc", [True, False])
+def test_a_mixed_batch_attends_as_on_the_cpu(tc, monkeypatch):
     """Decode, prefill and finetuning rows of one batch over the same codes: the model's attention on both devices.
 
     bf16 results (2^-8), and as many as the kernels' roundings move an average of values: 2^-7 of the largest."""
     from deltaserve_vllm_b200.models.decoder import ForwardBatch
+    monkeypatch.setattr(ops, "ATTN_TC", tc)
     arch = PRESETS["qwen3-test"]
     g = torch.Generator().manual_seed(5)
     hq, hkv, page = arch.num_heads, arch.num_kv_heads, 64
@@ -203,7 +205,7 @@ def test_a_mixed_batch_attends_as_on_the_cpu():
                          dec_block_tables=tables[:3].to(dev), dec_ctx_lens=i32(dec).to(dev), num_prefill_seqs=2,
                          pf_cu_q=i32([0, new[0], sum(new)]).to(dev), pf_ctx_lens=i32(contexts[3:]).to(dev),
                          pf_block_tables=tables[3:].contiguous().to(dev),
-                         ft_attn_tiles=ops.dense_attn_tiles(starts, ft, dev, bm=128), ft_lo=lo, ft_hi=lo + sum(ft))
+                         ft_attn_tiles=ops.dense_attn_tiles(starts, ft, dev, bm=128 if tc else 64), ft_lo=lo, ft_hi=lo + sum(ft))
         out = torch.full((lo + sum(ft), hq * 128), float("nan"), device=dev, dtype=dt)
         model.attention(0, qkv.to(dev, dt), out, b)
         return out.float().cpu()
@@ -212,3 +214,18 @@ def test_a_mixed_batch_attends_as_on_the_cpu():
     assert bool(((a - b).abs() <= b.abs() * 2 ** -8 + float(qkv.abs().max()) * 2 ** -7).all()), float((a - b).abs().max())
     rel = (a - b).norm(dim=1) / b.norm(dim=1)
     assert bool((rel <= 2 ** -7).all()), rel.max()
+
+
+def test_finetuning_rows_without_the_tcgen05_kernels(monkeypatch):
+    """DSV_ATTN_TC=0: finetuning samples over a 4-bit cache train on the warp-level kernels as well."""
+    monkeypatch.setattr(ops, "ATTN_TC", False)
+    ecfg = EngineConfig(model="qwen3-test", max_model_len=512, block_size=64, max_num_batched_tokens=512, max_loras=2,
+                        max_lora_rank=16, num_gpu_blocks_override=64, kv_cache_dtype="int4")
+    fcfg = FinetuneConfig(enable_finetuning=True, max_saved_finetuning_tokens=256, learning_rate=1e-3)
+    store = FinetuningStore.synthetic(4096, 8, 64, 100, seed=0, max_saved_finetuning_tokens=256, total_epochs=1)
+    eng = CoServingEngine(ecfg, fcfg, ft_store=store)
+    eng.add_request("r", list(range(40)), SamplingParams(max_tokens=4))
+    eng.run_until_idle(max_steps=2000)
+    eng.synchronize()
+    assert ops.check_device_error() == 0
+    assert eng.coord.completed_cycles >= 1 and all(l == l and l > 0 for l in eng.trainer.losses)
