@@ -268,6 +268,8 @@ def paged_decode4(q, cache, block_tables, ctx_lens, out, num_heads, scale):
 
 
 def copy_pages(caches, src, dst):
+    if any(c.shape != caches[0].shape or c.dtype != caches[0].dtype for c in caches):
+        raise ValueError("copy_pages: caches must be contiguous tensors of one shape and element size on one device")
     src, dst = torch.as_tensor(src), torch.as_tensor(dst)
     for c in caches:
         c[dst.to(c.device)] = c[src.to(c.device)]

@@ -144,3 +144,12 @@ def test_query_heads_are_1_to_16_times_the_kv_heads(heads):
         ops.paged_decode4(q, cache, tables, one, q.clone(), heads, 1.0, None)
     with pytest.raises(ValueError):
         ops.paged_prefill4(q, cache, tables, cu, one, q.clone(), heads, 1.0, None)
+
+
+def test_copy_pages_refuses_caches_that_differ():
+    """As on the GPU: nothing is copied when the caches have not one shape."""
+    caches = [torch.zeros(6, 2, 3), torch.ones(4, 2, 3)]
+    before = [c.clone() for c in caches]
+    with pytest.raises(ValueError):
+        ops.copy_pages(caches, [0], [5])
+    assert all(torch.equal(a, b) for a, b in zip(caches, before))
